@@ -1,0 +1,284 @@
+// capi_fp8.cu — the extern "C" boundary of routing from logits and of the 8-bit (e4m3) layers: argument
+// checks, the workspace's layout, and the order of the launches.  Nothing here allocates or synchronises.
+#include <cstdint>
+
+#include <cuda_runtime.h>
+
+#include "exl3_internal.h"
+#include "../../include/exl3_b200.h"
+
+using namespace exl3b;
+
+namespace {
+
+cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+int64_t up256(int64_t n) { return (n + 255) & ~int64_t(255); }
+int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+bool is_dtype(int64_t d) { return d >= EXL3_DTYPE_F32 && d <= EXL3_DTYPE_BF16; }
+
+constexpr int64_t kMaxDim = 0x7fffff00;
+
+// A piece of the caller's workspace, 256-byte aligned.
+struct Carver {
+    uint8_t* base;
+    int64_t used = 0;
+    template <class T> T* take(int64_t n)
+    {
+        uint8_t* p = base ? base + used : nullptr;
+        used += up256(n * (int64_t) sizeof(T));
+        return reinterpret_cast<T*>(p);
+    }
+};
+
+// Quantised rows: e4m3 [rows, k] and scales [k / 128][rows], so that a K block's scales lie side by side.
+struct Rows8 {
+    uint8_t* q;
+    float* s;
+};
+
+Rows8 take_rows(Carver& c, int64_t rows, int64_t k)
+{
+    Rows8 r;
+    r.q = c.take<uint8_t>(rows * k);
+    r.s = c.take<float>(rows * blocks128(k));
+    return r;
+}
+
+struct ExpertBuffers {
+    int64_t* slot;
+    void* weight_sorted;
+    int32_t *expert_of_row, *counts, *row0, *meta, *scratch;
+    Rows8 x, h;
+    float* y;
+};
+
+ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_t d, int64_t f)
+{
+    const int64_t R = T * topk;
+    ExpertBuffers b{};
+    b.slot = c.take<int64_t>(R);
+    b.weight_sorted = c.take<uint16_t>(R);
+    b.expert_of_row = c.take<int32_t>(R);
+    b.counts = c.take<int32_t>(E);
+    b.row0 = c.take<int32_t>(E);
+    b.meta = c.take<int32_t>(2);
+    b.scratch = c.take<int32_t>(route_sort_scratch_elems(R, (int) E));
+    b.x = take_rows(c, R, d);
+    b.h = take_rows(c, R, f);
+    b.y = c.take<float>(R * d);
+    return b;
+}
+
+int check_rows(const char* what, int64_t dtype, int64_t rows, int64_t K, int64_t stride)
+{
+    if (!is_dtype(dtype)) return set_error("%s: unknown dtype", what);
+    if (rows < 0 || rows > kMaxDim) return set_error("%s: invalid row count", what);
+    if (K < 1 || K > kMaxDim) return set_error("%s: invalid row length", what);
+    if (rows > 1 && stride < K) return set_error("%s: rows overlap (row stride below the row length)", what);
+    return EXL3_OK;
+}
+
+int check_experts_shape(const char* what, int64_t T, int64_t topk, int64_t E, int64_t d, int64_t f)
+{
+    if (E <= 0 || E > kMaxExperts) return set_error("too many experts");
+    if (topk < 1 || topk > 32) return set_error("%s: topk must be 1..32", what);
+    if (T < 0 || T > kMaxDim || T * topk > kMaxDim) return set_error("invalid routing shape");
+    if (d <= 0 || d % 128 != 0 || d > (1 << 24)) return set_error("%s: d must be a multiple of 128", what);
+    if (f <= 0 || f % 128 != 0 || f > (1 << 24)) return set_error("%s: f must be a multiple of 128", what);
+    return EXL3_OK;
+}
+
+int check_out(const char* what, const void* out, int64_t out_dtype, int64_t T, int64_t n, int64_t stride)
+{
+    if (!is_dtype(out_dtype)) return set_error("%s: unknown output dtype", what);
+    if (T > 1 && stride < n) return set_error("%s: output rows overlap", what);
+    if (!out) return set_error("tensors must be CUDA");
+    return EXL3_OK;
+}
+
+// Both products of the gated MLP over quantised rows x [rows, d]: gate | up into h, then down into `out`.
+int run_mlp(const Rows8& x, const Rows8& h, int64_t rows, int64_t d, int64_t f, int64_t E, const int32_t* counts,
+            const int32_t* row0, const void* w13, const float* w13_scale, const void* w2, const float* w2_scale,
+            double limit, void* out, int64_t out_stride, int64_t out_dtype, int accumulate, const int64_t* slot,
+            int32_t* status, cudaStream_t stream)
+{
+    Fp8GemmProblem p{};
+    p.x = x.q; p.rows = rows; p.x_stride = d; p.K = (int) d;
+    p.sx = x.s; p.sx_row = 1; p.sx_blk = rows;
+    p.w = w13; p.w_stride = d; p.w_expert = 2 * f * d; p.N = (int) (2 * f); p.n_experts = (int) E;
+    p.sw = w13_scale; p.sw_n = blocks128(d); p.sw_expert = blocks128(2 * f) * p.sw_n;
+    p.counts = counts; p.row0 = row0;
+    p.swiglu = 1; p.limit = (float) limit;
+    p.h = h.q; p.h_stride = f; p.hs = h.s; p.hs_row = 1; p.hs_blk = rows;
+    p.status = status;
+    int rc = launch_fp8_gemm(p, stream);
+    if (rc) return rc;
+    Fp8GemmProblem q{};
+    q.x = h.q; q.rows = rows; q.x_stride = f; q.K = (int) f;
+    q.sx = h.s; q.sx_row = 1; q.sx_blk = rows;
+    q.w = w2; q.w_stride = f; q.w_expert = d * f; q.N = (int) d; q.n_experts = (int) E;
+    q.sw = w2_scale; q.sw_n = blocks128(f); q.sw_expert = blocks128(d) * q.sw_n;
+    q.counts = counts; q.row0 = row0;
+    q.out = out; q.out_stride = out_stride; q.out_dtype = (int) out_dtype; q.accumulate = accumulate;
+    q.slot = slot; q.status = status;
+    return launch_fp8_gemm(q, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int exl3_route_logits(const void* logits, int64_t dtype, int64_t T, int64_t E, int64_t row_stride, const float* bias,
+                      int64_t softmax, int64_t n_group, int64_t topk_group, int64_t group_top, int64_t topk,
+                      int64_t norm, double scale, int64_t* ids, float* weights, void* stream)
+{
+    if (!is_dtype(dtype)) return set_error("route_logits: logits must be float32, float16 or bfloat16");
+    if (E <= 0 || E > kMaxExperts) return set_error("too many experts");
+    if (T < 0 || T > kMaxDim) return set_error("invalid routing shape");
+    if (T > 1 && row_stride < E) return set_error("route_logits: rows overlap (row stride below the number of experts)");
+    if (n_group < 1 || n_group > 32 || E % n_group != 0)
+        return set_error("route_logits: n_group must be 1..32 and divide the number of experts");
+    if (topk_group < 1 || topk_group > n_group) return set_error("route_logits: topk_group must be 1..n_group");
+    if (group_top < 1 || group_top > 2 || group_top > E / n_group)
+        return set_error("route_logits: group_top must be 1 or 2 and at most the experts of a group");
+    if (topk < 1 || topk > 32 || topk > topk_group * (E / n_group))
+        return set_error("route_logits: topk must be 1..32 and at most the experts of the kept groups");
+    if (!(scale >= -3.0e38 && scale <= 3.0e38)) return set_error("route_logits: scale must be finite");
+    if (T == 0) return EXL3_OK;
+    if (!logits || !ids || !weights) return set_error("tensors must be CUDA");
+    return launch_route_logits(logits, (int) dtype, T, (int) E, row_stride, bias, softmax ? 1 : 0, (int) n_group,
+                               (int) topk_group, (int) group_top, (int) topk, norm ? 1 : 0, (float) scale, ids, weights,
+                               as_stream(stream));
+}
+
+int exl3_fp8_quantize_rows(const void* x, int64_t dtype, int64_t rows, int64_t K, int64_t x_stride, int64_t pow2,
+                           void* q, int64_t q_stride, float* scale, int64_t s_row, int64_t s_blk, void* stream)
+{
+    const int rc = check_rows("fp8_quantize_rows", dtype, rows, K, x_stride);
+    if (rc) return rc;
+    if (rows > 1 && q_stride < K) return set_error("fp8_quantize_rows: output rows overlap");
+    if (rows == 0) return EXL3_OK;
+    if (!x || !q || !scale) return set_error("tensors must be CUDA");
+    return launch_fp8_quantize(x, (int) dtype, rows, (int) K, x_stride, pow2 ? 1 : 0, q, q_stride, scale, s_row, s_blk,
+                               nullptr, 1, nullptr, as_stream(stream));
+}
+
+int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K)
+{
+    if (T < 0 || T > kMaxDim || K < 16 || K % 16 != 0 || K > (1 << 24)) return -1;
+    Carver c{nullptr};
+    take_rows(c, T, K);
+    return c.used;
+}
+
+int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t x_stride, const void* w, int64_t w_stride,
+                    const float* w_scale, int64_t w_scale_stride, int64_t N, void* out, int64_t out_dtype,
+                    int64_t out_stride, int accumulate, void* workspace, int64_t workspace_bytes, int32_t* status,
+                    void* stream)
+{
+    int rc = check_rows("fp8_linear", dtype, T, K, x_stride);
+    if (rc) return rc;
+    if (K % 16 != 0 || K > (1 << 24)) return set_error("fp8_linear: K must be a multiple of 16");
+    if (N < 1 || N > (1 << 24)) return set_error("fp8_linear: invalid number of weight rows");
+    if (T == 0) return EXL3_OK;
+    if ((rc = check_out("fp8_linear", out, out_dtype, T, N, out_stride))) return rc;
+    if (!x || !w || !w_scale || !workspace) return set_error("tensors must be CUDA");
+    if (!aligned16(w) || w_stride % 16 != 0 || w_stride < K)
+        return set_error("fp8_linear: the weight's rows must be 16-byte aligned");
+    if (w_scale_stride < blocks128(K)) return set_error("fp8_linear: weight scales [ceil(N / 128), ceil(K / 128)]");
+    if (!aligned16(workspace) || workspace_bytes < exl3_fp8_linear_workspace(T, K))
+        return set_error("fp8_linear: workspace must hold exl3_fp8_linear_workspace() bytes");
+    Carver c{static_cast<uint8_t*>(workspace)};
+    const Rows8 r = take_rows(c, T, K);
+    rc = launch_fp8_quantize(x, (int) dtype, T, (int) K, x_stride, 0, r.q, K, r.s, 1, T, nullptr, 1, nullptr,
+                             as_stream(stream));
+    if (rc) return rc;
+    Fp8GemmProblem p{};
+    p.x = r.q; p.rows = T; p.x_stride = K; p.K = (int) K;
+    p.sx = r.s; p.sx_row = 1; p.sx_blk = T;
+    p.w = w; p.w_stride = w_stride; p.w_expert = w_stride * N; p.N = (int) N; p.n_experts = 1;
+    p.sw = w_scale; p.sw_n = w_scale_stride; p.sw_expert = 0;
+    p.out = out; p.out_stride = out_stride; p.out_dtype = (int) out_dtype; p.accumulate = accumulate ? 1 : 0;
+    p.status = status;
+    return launch_fp8_gemm(p, as_stream(stream));
+}
+
+int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f)
+{
+    if (T < 0 || T > kMaxDim || d <= 0 || d % 128 != 0 || d > (1 << 24) || f <= 0 || f % 128 != 0 || f > (1 << 24))
+        return -1;
+    Carver c{nullptr};
+    take_rows(c, T, d);
+    take_rows(c, T, f);
+    return c.used;
+}
+
+int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_stride, const void* w13,
+                 const float* w13_scale, const void* w2, const float* w2_scale, int64_t f, double limit, void* out,
+                 int64_t out_dtype, int64_t out_stride, int accumulate, void* workspace, int64_t workspace_bytes,
+                 int32_t* status, void* stream)
+{
+    int rc = check_rows("fp8_mlp", dtype, T, d, x_stride);
+    if (rc || (rc = check_experts_shape("fp8_mlp", T, 1, 1, d, f))) return rc;
+    if (!(limit > 0.0)) return set_error("fp8_mlp: limit must be positive");
+    if (T == 0) return EXL3_OK;
+    if ((rc = check_out("fp8_mlp", out, out_dtype, T, d, out_stride))) return rc;
+    if (!x || !w13 || !w13_scale || !w2 || !w2_scale || !workspace) return set_error("tensors must be CUDA");
+    if (!aligned16(w13) || !aligned16(w2)) return set_error("fp8_mlp: weights must be 16-byte aligned");
+    if (!aligned16(workspace) || workspace_bytes < exl3_fp8_mlp_workspace(T, d, f))
+        return set_error("fp8_mlp: workspace must hold exl3_fp8_mlp_workspace() bytes");
+    Carver c{static_cast<uint8_t*>(workspace)};
+    const Rows8 xr = take_rows(c, T, d), hr = take_rows(c, T, f);
+    rc = launch_fp8_quantize(x, (int) dtype, T, (int) d, x_stride, 0, xr.q, d, xr.s, 1, T, nullptr, 1, nullptr,
+                             as_stream(stream));
+    if (rc) return rc;
+    return run_mlp(xr, hr, T, d, f, 1, nullptr, nullptr, w13, w13_scale, w2, w2_scale, limit, out, out_stride,
+                   out_dtype, accumulate ? 1 : 0, nullptr, status, as_stream(stream));
+}
+
+int64_t exl3_fp8_experts_workspace(int64_t T, int64_t topk, int64_t E, int64_t d, int64_t f)
+{
+    if (check_experts_shape("fp8_experts", T, topk, E, d, f)) return -1;
+    Carver c{nullptr};
+    take_experts(c, T, topk, E, d, f);
+    return c.used;
+}
+
+int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_stride, const void* ids,
+                     int ids_is_int64, const void* weights, int64_t weight_dtype, int64_t topk, int64_t E,
+                     const void* w13, const float* w13_scale, const void* w2, const float* w2_scale, int64_t f,
+                     double limit, void* out, int64_t out_dtype, int64_t out_stride, int accumulate, void* workspace,
+                     int64_t workspace_bytes, int32_t* status, void* stream)
+{
+    int rc = check_rows("fp8_experts", dtype, T, d, x_stride);
+    if (rc || (rc = check_experts_shape("fp8_experts", T, topk, E, d, f))) return rc;
+    if (!is_dtype(weight_dtype)) return set_error("unknown weight dtype");
+    if (!(limit > 0.0)) return set_error("fp8_experts: limit must be positive");
+    if (T == 0) return EXL3_OK;
+    if ((rc = check_out("fp8_experts", out, out_dtype, T, d, out_stride))) return rc;
+    if (!x || !ids || !weights || !w13 || !w13_scale || !w2 || !w2_scale || !workspace)
+        return set_error("tensors must be CUDA");
+    if (!aligned16(w13) || !aligned16(w2)) return set_error("fp8_experts: weights must be 16-byte aligned");
+    if (!aligned16(workspace) || workspace_bytes < exl3_fp8_experts_workspace(T, topk, E, d, f))
+        return set_error("fp8_experts: workspace must hold exl3_fp8_experts_workspace() bytes");
+    Carver c{static_cast<uint8_t*>(workspace)};
+    const ExpertBuffers b = take_experts(c, T, topk, E, d, f);
+    const int64_t R = T * topk;
+    cudaStream_t st = as_stream(stream);
+    // sorted by routing slot t * topk + j, so that each row knows both its token and its place in y
+    rc = launch_route_sort(ids, ids_is_int64 ? 1 : 0, weights, (int) weight_dtype, R, 1, (int) E, 0, b.slot,
+                           b.weight_sorted, b.expert_of_row, b.counts, b.row0, nullptr, nullptr, b.meta, nullptr,
+                           b.scratch, st);
+    if (rc) return rc;
+    rc = launch_fp8_quantize(x, (int) dtype, R, (int) d, x_stride, 0, b.x.q, d, b.x.s, 1, R, b.slot, (int) topk,
+                             b.meta + 1, st);
+    if (rc) return rc;
+    rc = run_mlp(b.x, b.h, R, d, f, E, b.counts, b.row0, w13, w13_scale, w2, w2_scale, limit, b.y, d, EXL3_DTYPE_F32, 0,
+                 b.slot, status, st);
+    if (rc) return rc;
+    return launch_fp8_combine(b.y, d, ids, ids_is_int64 ? 1 : 0, weights, (int) weight_dtype, T, (int) topk, (int) E,
+                              (int) d, accumulate ? 1 : 0, out, (int) out_dtype, out_stride, st);
+}
+
+}  // extern "C"

@@ -153,6 +153,48 @@ struct GemmProblem {
 };
 
 int launch_trellis_gemm(const GemmProblem& p, cudaStream_t stream);
+
+// ---- route_logits.cu (dtype codes as EXL3_DTYPE_*)
+int launch_route_logits(const void* logits, int dtype, int64_t T, int E, int64_t row_stride, const float* bias,
+                        int softmax, int n_group, int topk_group, int group_top, int topk, int norm, float scale,
+                        int64_t* ids, float* weights, cudaStream_t stream);
+
+// ---- fp8_rows.cu
+// slot (nullable): row r is x[slot[r] / topk]; rows_dev (nullable): only min(rows, *rows_dev) rows exist.
+int launch_fp8_quantize(const void* x, int dtype, int64_t rows, int K, int64_t x_stride, int pow2, void* q,
+                        int64_t q_stride, float* scale, int64_t s_row, int64_t s_blk, const int64_t* slot, int topk,
+                        const int32_t* rows_dev, cudaStream_t stream);
+int launch_fp8_combine(const float* y, int64_t y_stride, const void* ids, int ids_i64, const void* weights, int wdtype,
+                       int64_t T, int topk, int E, int d, int accumulate, void* out, int out_dtype, int64_t out_stride,
+                       cudaStream_t stream);
+
+// ---- fp8_gemm.cu
+struct Fp8GemmProblem {
+    const void* x;                 // e4m3 [rows, K], row stride x_stride bytes (a multiple of 16)
+    int64_t rows, x_stride;
+    int K;
+    const float* sx;               // scales of x: element strides sx_row, sx_blk
+    int64_t sx_row, sx_blk;
+    const void* w;                 // e4m3 [n_experts, N, K], strides in bytes (multiples of 16)
+    int64_t w_stride, w_expert;
+    int N, n_experts;
+    const float* sw;               // [n_experts, N / 128, K / 128], the last dimension contiguous
+    int64_t sw_expert, sw_n;
+    const int32_t* counts;         // [n_experts] rows of each expert and the first of them, or null (one
+    const int32_t* row0;           //  expert with all rows)
+    int swiglu;                    // 0: store, 1: gate | up halves of N -> quantised rows
+    void* out;                     // store: dtype code out_dtype, element stride out_stride
+    int64_t out_stride;
+    int out_dtype, accumulate;
+    const int64_t* slot;           // store: output row of row r, or null
+    float limit;                   // swiglu: e4m3 rows [rows, N / 2] and their scales
+    void* h;
+    int64_t h_stride;
+    float* hs;
+    int64_t hs_row, hs_blk;
+    int32_t* status;
+};
+int launch_fp8_gemm(const Fp8GemmProblem& p, cudaStream_t stream);
 int trellis_gemm_smem_bytes();
 
 }  // namespace exl3b

@@ -1,0 +1,204 @@
+// fp8_rows.cu — the row kernels of the 8-bit layers: quantising rows, and summing a token's routes.
+#include "fp8_common.cuh"
+
+namespace exl3b {
+
+namespace {
+
+using namespace fp8;
+
+// ------------------------------------------------------------------------------------ quantised rows
+//     s[r, b] = max(max_k |x[r, k]|, 2^-64) / 448   (or the least power of two at or above that)
+//     q[r, k] = e4m3(x[r, k] / s[r, k / 128])       b = k / 128
+// bound by bytes: a row is read once (2 or 4 bytes a value) and written once (1 byte).  Eight lanes hold a block,
+// 16 values each, so loads are 32 or 64 bytes and the store 16 bytes a lane, and a block's maximum is three shuffles.
+struct QuantArgs {
+    const void* x;
+    int64_t x_stride;                // elements
+    int K, n_blocks;
+    int pow2;
+    uint8_t* q;
+    int64_t q_stride;
+    float* scale;
+    int64_t s_row, s_blk;            // element strides of the scales
+    int64_t rows;
+    // gather (optional): row r holds x[slot[r] / topk]; only the first *rows_dev rows exist
+    const int64_t* slot;
+    int topk;
+    const int32_t* rows_dev;
+};
+
+constexpr int Q_THREADS = 256;
+
+template <class T, bool VEC>
+__global__ __launch_bounds__(Q_THREADS)
+void quantize_rows_kernel(const QuantArgs p)
+{
+    const int lane8 = threadIdx.x & 7;
+    const int64_t rows = p.rows_dev ? min(p.rows, (int64_t) *p.rows_dev) : p.rows;
+    const int64_t units = rows * p.n_blocks;                        // (row, block) pairs, blocks fastest
+    const int64_t step = (int64_t) gridDim.x * (Q_THREADS / 8);
+    // whole warps take part in the shuffles: the bound is rounded up to the warp's four units
+    const int64_t first = ((int64_t) blockIdx.x * Q_THREADS + threadIdx.x) >> 3;
+    for (int64_t u = first; u - (first & 3) < units; u += step)
+    {
+        const bool live = u < units;
+        const int64_t r = live ? u / p.n_blocks : 0;
+        const int b = live ? (int) (u - r * p.n_blocks) : 0;
+        const int64_t src = p.slot && live ? __ldg(p.slot + r) / p.topk : r;
+        const int k0 = b * kBlock + lane8 * 16;
+        const T* x = reinterpret_cast<const T*>(p.x) + src * p.x_stride + k0;
+        float v[16];
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+        if (live)
+        {
+            if (VEC)                                                // K % 16 == 0, rows 16-byte aligned
+            {
+                if (k0 < p.K)
+                {
+                    constexpr int PER = 16 / sizeof(T);
+                    #pragma unroll
+                    for (int j = 0; j < 16 / PER; ++j)
+                    {
+                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(x) + j);
+                        const T* h = reinterpret_cast<const T*>(&w);
+                        #pragma unroll
+                        for (int i = 0; i < PER; ++i) v[j * PER + i] = to_float(h[i]);
+                    }
+                }
+            }
+            else
+            {
+                #pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (k0 + i < p.K) v[i] = to_float(x[i]);
+            }
+        }
+        uint32_t m = 0;                                             // magnitudes as integers: NaN is the largest
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        #pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!live) continue;
+        const float s = block_scale(__uint_as_float(m), p.pow2 != 0);
+        const float inv = 1.0f / s;
+        uint32_t w[4];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            float f[4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = quotient(v[4 * j + i], s, inv);
+            w[j] = to_e4m3x2(f[0], f[1]) | to_e4m3x2(f[2], f[3]) << 16;
+        }
+        uint8_t* q = p.q + r * p.q_stride + k0;
+        if (VEC)
+        {
+            if (k0 < p.K) *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        else
+        {
+            #pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (k0 + i < p.K) q[i] = (uint8_t) (w[i >> 2] >> (8 * (i & 3)));
+        }
+        if (lane8 == 0) p.scale[r * p.s_row + b * p.s_blk] = s;
+    }
+}
+
+// ------------------------------------------------------------------------------------ sum over a token's routes
+//     out[t] = (accumulate ? out[t] : 0) + sum over j ascending, ids[t, j] in [0, E), of w[t, j] * y[t * topk + j]
+// in fp32 and a fixed order (no atomics), rounded once to out's type.  Bound by reading y.
+struct CombineArgs {
+    const float* y;
+    int64_t y_stride;
+    const void* ids;
+    int ids_i64;
+    const void* weights;
+    int wdtype;
+    int64_t T;
+    int topk, E, d, accumulate;
+    void* out;
+    int64_t out_stride;
+};
+
+__device__ __forceinline__ float route_weight(const void* w, int dtype, int64_t i)
+{
+    if (dtype == 0) return __ldg(reinterpret_cast<const float*>(w) + i);
+    if (dtype == 1) return __half2float(reinterpret_cast<const __half*>(w)[i]);
+    return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(w)[i]);
+}
+
+template <class To>
+__global__ __launch_bounds__(256)
+void combine_routes_kernel(const CombineArgs p)
+{
+    const int64_t t = blockIdx.y + (int64_t) blockIdx.z * 65535;
+    if (t >= p.T) return;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (c >= p.d) return;                                           // d % 4 == 0
+    To* out = reinterpret_cast<To*>(p.out) + t * p.out_stride + c;
+    float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.accumulate)
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = to_float(out[i]);
+    for (int j = 0; j < p.topk; ++j)
+    {
+        const int64_t s = t * p.topk + j;
+        const int64_t e = p.ids_i64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + s)
+                                    : (int64_t) __ldg(reinterpret_cast<const int*>(p.ids) + s);
+        if (e < 0 || e >= p.E) continue;
+        const float w = route_weight(p.weights, p.wdtype, s);
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p.y + s * p.y_stride + c));
+        a[0] = fmaf(w, v.x, a[0]);
+        a[1] = fmaf(w, v.y, a[1]);
+        a[2] = fmaf(w, v.z, a[2]);
+        a[3] = fmaf(w, v.w, a[3]);
+    }
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = from_float<To>(a[i]);
+}
+
+template <class T>
+void launch_quant(const QuantArgs& p, bool vec, unsigned grid, cudaStream_t stream)
+{
+    if (vec) quantize_rows_kernel<T, true><<<grid, Q_THREADS, 0, stream>>>(p);
+    else quantize_rows_kernel<T, false><<<grid, Q_THREADS, 0, stream>>>(p);
+}
+
+}  // namespace
+
+int launch_fp8_quantize(const void* x, int dtype, int64_t rows, int K, int64_t x_stride, int pow2, void* q,
+                        int64_t q_stride, float* scale, int64_t s_row, int64_t s_blk, const int64_t* slot, int topk,
+                        const int32_t* rows_dev, cudaStream_t stream)
+{
+    QuantArgs p{};
+    p.x = x; p.x_stride = x_stride; p.K = K; p.n_blocks = (K + kBlock - 1) / kBlock; p.pow2 = pow2;
+    p.q = static_cast<uint8_t*>(q); p.q_stride = q_stride; p.scale = scale; p.s_row = s_row; p.s_blk = s_blk;
+    p.rows = rows; p.slot = slot; p.topk = topk; p.rows_dev = rows_dev;
+    const int64_t size = dtype == 0 ? 4 : 2;
+    const bool vec = K % 16 == 0 && (x_stride * size) % 16 == 0 && q_stride % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    const int64_t ctas = (rows * p.n_blocks + Q_THREADS / 8 - 1) / (Q_THREADS / 8);
+    const int64_t most = (int64_t) device_sm_count() * 64;
+    const unsigned grid = (unsigned) (ctas < most ? ctas : most);
+    if (dtype == 0) launch_quant<float>(p, vec, grid, stream);
+    else if (dtype == 1) launch_quant<__half>(p, vec, grid, stream);
+    else launch_quant<__nv_bfloat16>(p, vec, grid, stream);
+    return check_launch("fp8_quantize_rows");
+}
+
+int launch_fp8_combine(const float* y, int64_t y_stride, const void* ids, int ids_i64, const void* weights, int wdtype,
+                       int64_t T, int topk, int E, int d, int accumulate, void* out, int out_dtype, int64_t out_stride,
+                       cudaStream_t stream)
+{
+    CombineArgs p{y, y_stride, ids, ids_i64, weights, wdtype, T, topk, E, d, accumulate, out, out_stride};
+    const dim3 grid((unsigned) ((d / 4 + 255) / 256), (unsigned) (T < 65535 ? T : 65535), (unsigned) ((T + 65534) / 65535));
+    if (out_dtype == 0) combine_routes_kernel<float><<<grid, 256, 0, stream>>>(p);
+    else if (out_dtype == 1) combine_routes_kernel<__half><<<grid, 256, 0, stream>>>(p);
+    else combine_routes_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
+    return check_launch("fp8_combine");
+}
+
+}  // namespace exl3b

@@ -21,6 +21,7 @@ from __future__ import annotations
 import torch
 
 import b200_ext
+import exl3_fp8
 import exl3_grouped_runtime as rt
 
 
@@ -61,7 +62,16 @@ def exl3_linear(x2d: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, svh
 
 def dense_mlp_prefill(x2d: torch.Tensor, mlp, limit: float, out: torch.Tensor | None = None,
                       stage_hook=None) -> torch.Tensor:
-    """SwiGLU MLP in the stacked layout with one expert -> fp32 [T, d] (added into `out` if given)."""
+    """SwiGLU MLP in the stacked layout with one expert -> fp32 [T, d] (added into `out` if given).  An 8-bit
+    MLP (w13_fp8 ..., exl3_fp8) is one call; its hook sees "fp8_mlp" and "end"."""
+    if exl3_fp8.is_fp8_layer(mlp):
+        hook = stage_hook if stage_hook is not None else (lambda name: None)
+        hook("fp8_mlp")
+        if out is not None and out.dtype != torch.float32:
+            raise RuntimeError("dense_mlp_prefill: out must be fp32")
+        out = exl3_fp8.fp8_mlp_prefill(x2d, mlp, limit, out=out)
+        hook("end")
+        return out
     if int(mlp.w13_trellis.shape[0]) != 1:
         raise RuntimeError("dense_mlp_prefill: the MLP must be stored as one expert ([1, ...] tensors)")
     T = x2d.shape[0]

@@ -73,6 +73,14 @@ def grouped_prefill(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     and with "end" after the last one (used to record CUDA events between kernels).  `out` (fp32 [T, K],
     contiguous), if given, is added into; otherwise a new tensor is returned."""
     hook = stage_hook if stage_hook is not None else (lambda name: None)
+    if getattr(layer, "w13_fp8", None) is not None:         # 8-bit experts: one call, always in a fixed order
+        import exl3_fp8
+        if out is not None and out.dtype != torch.float32:
+            raise RuntimeError("out must be a contiguous fp32 [T, K] tensor on the input's device")
+        hook("fp8_experts")
+        out = exl3_fp8.fp8_prefill(x2d, ids, weights, layer, limit, out=out)
+        hook("end")
+        return out
     if deterministic is None:
         deterministic = deterministic_default()
     gp = _load_ext()

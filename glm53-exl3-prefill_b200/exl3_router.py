@@ -41,6 +41,43 @@ class NoauxTcRouter:
         return ids, w
 
 
+class LogitsRouter:
+    """Routing from router logits, for callers that compute them (any router module): sigmoid or softmax
+    scores, an optional selection bias [E], groups of experts, renormalised and scaled weights.
+
+    With c = score + bias: a group's score is the sum of its `group_top` largest c; the topk experts by c
+    inside the `topk_group` best of `n_group` groups are chosen, best first, ties to the lower id.  Masked
+    experts (logit -inf or NaN) are never chosen; a token with fewer than topk left gets id -1, weight 0."""
+
+    def __init__(self, topk: int, scoring: str = "sigmoid", bias: torch.Tensor | None = None, n_group: int = 1,
+                 topk_group: int = 1, group_top: int = 2, norm: bool = True, scale: float = 1.0):
+        if scoring not in ("sigmoid", "softmax"):
+            raise RuntimeError("LogitsRouter: scoring must be \"sigmoid\" or \"softmax\"")
+        self.topk, self.softmax, self.norm, self.scale = int(topk), scoring == "softmax", bool(norm), float(scale)
+        self.n_group, self.topk_group, self.group_top = int(n_group), int(topk_group), int(group_top)
+        self.bias = None if bias is None else bias.to(dtype=torch.float32).contiguous()
+
+    def route(self, logits: torch.Tensor):
+        """logits [T, E] (fp32, fp16 or bf16; rows may be strided) -> (ids int64 [T, topk], weights fp32 [T, topk])."""
+        if logits.dim() != 2:
+            raise RuntimeError("LogitsRouter: logits must be [T, E]")
+        ids = torch.empty(logits.shape[0], self.topk, dtype=torch.int64, device=logits.device)
+        w = torch.empty(logits.shape[0], self.topk, dtype=torch.float32, device=logits.device)
+        b200_ext.route_logits(logits, self.bias, self.topk, self.softmax, self.n_group, self.topk_group,
+                              self.group_top, self.norm, self.scale, ids, w)
+        return ids, w
+
+
+def moe_prefill_from_logits(x2d: torch.Tensor, logits: torch.Tensor, router: LogitsRouter, layer, limit: float,
+                            shared=None, return_routing: bool = False):
+    """Hidden states [T, d] and their router logits [T, E] -> routed experts (+ the shared expert if given), fp32
+    [T, d]; trellis and 8-bit layers alike.  With return_routing, also returns (ids, weights)."""
+    import exl3_dense
+    ids, w = router.route(logits)
+    out = exl3_dense.moe_block_prefill(x2d, ids, w, layer, shared, limit)
+    return (out, ids, w) if return_routing else out
+
+
 def moe_prefill_from_hidden(x2d: torch.Tensor, router: NoauxTcRouter, layer, limit: float, shared=None,
                             stage_hook=None, return_routing: bool = False, deterministic: bool | None = None):
     """Hidden states [T, d] -> routed-expert output fp32 [T, d] (+ the shared expert if given), with the

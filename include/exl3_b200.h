@@ -42,7 +42,7 @@ extern "C" {
 #define EXL3_ERR_WAIT_TIMEOUT 1
 #define EXL3_ERR_INVALID_EXPERT 2
 
-/* weight dtype codes for exl3_route_sort */
+/* dtype codes: route weights (exl3_route_sort), activations and outputs of the 8-bit layers */
 #define EXL3_DTYPE_F32 0
 #define EXL3_DTYPE_F16 1
 #define EXL3_DTYPE_BF16 2
@@ -225,6 +225,62 @@ EXL3_API int exl3_fat_gemm_scatter(const void* a, int64_t size_m, int64_t size_k
                           int64_t size_n, float* out, int64_t out_rows, const void* svh,
                           const int64_t* token_idx, const void* route_weight, int64_t K, int mcg, int mul1,
                           int32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Routing from router logits.  No reference counterpart (the reference receives topk_ids / topk_weights
+ * from vLLM's router).  For every token, with logits l[E] and an optional bias b[E]:
+ *   s = sigmoid(l), or softmax(l) if `softmax`;   c = s + b;
+ *   a group's score is the sum of its group_top (1 or 2) largest c, over n_group equal groups of consecutive experts;
+ *   ids = the topk experts by c inside the topk_group groups with the largest scores, best first;
+ *   weights = s[ids] / (sum + 1e-20) if norm else s[ids], times scale.
+ * Ties go to the lower expert (group), and the choice is that of exact arithmetic.  NaN and -inf logits are
+ * masked (never chosen); missing experts give id -1 and weight 0.  logits [T, E] of `dtype` with element
+ * stride row_stride between rows, bias fp32 [E] (finite) or NULL, ids int64 / weights fp32 [T, topk].
+ * E <= 1024, n_group <= 32, topk <= 32.
+ * ------------------------------------------------------------------------------------------- */
+EXL3_API int exl3_route_logits(const void* logits, int64_t dtype, int64_t T, int64_t E, int64_t row_stride,
+                               const float* bias, int64_t softmax, int64_t n_group, int64_t topk_group,
+                               int64_t group_top, int64_t topk, int64_t norm, double scale, int64_t* ids,
+                               float* weights, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * 8-bit layers (no reference counterpart): weights in e4m3 with one fp32 scale per block of 128 x 128, the
+ * activations quantised to e4m3 with one fp32 scale per row and 128 columns:
+ *   s = max(|x| over the block, 2^-64) / 448 (pow2: the least power of two at or above that), q = e4m3(x / s).
+ * A block that holds NaN or inf gives NaN.  dtype codes: EXL3_DTYPE_*; strides in elements.
+ * ------------------------------------------------------------------------------------------- */
+
+/* q e4m3 [rows, K] (row stride q_stride), scale fp32: block b of row r at scale[r * s_row + b * s_blk]. */
+EXL3_API int exl3_fp8_quantize_rows(const void* x, int64_t dtype, int64_t rows, int64_t K, int64_t x_stride,
+                                    int64_t pow2, void* q, int64_t q_stride, float* scale, int64_t s_row,
+                                    int64_t s_blk, void* stream);
+
+/* out [T, N] = quantised(x) . W^T (added to out if accumulate).  W e4m3 [N, K] (row stride w_stride, 16-byte
+ * aligned rows), w_scale [ceil(N / 128), ceil(K / 128)] with row stride w_scale_stride.  K % 16 == 0. */
+EXL3_API int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K);      /* bytes; -1: bad arguments */
+EXL3_API int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t x_stride, const void* w,
+                             int64_t w_stride, const float* w_scale, int64_t w_scale_stride, int64_t N, void* out,
+                             int64_t out_dtype, int64_t out_stride, int accumulate, void* workspace,
+                             int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* A gated MLP: out [T, d] (+)= quantised( silu(min(g, limit)) * clamp(u, -limit, limit) ) . w2^T with
+ * g | u = quantised(x) . w13^T.  w13 e4m3 [2f, d] (gate rows, then up rows), w2 e4m3 [d, f], contiguous, scales
+ * [2f / 128, d / 128] and [d / 128, f / 128].  d, f % 128 == 0. */
+EXL3_API int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f);
+EXL3_API int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_stride, const void* w13,
+                          const float* w13_scale, const void* w2, const float* w2_scale, int64_t f, double limit,
+                          void* out, int64_t out_dtype, int64_t out_stride, int accumulate, void* workspace,
+                          int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* Routed experts: out[t] (+)= sum over j ascending of weights[t, j] * mlp_{ids[t, j]}(x[t]), in fp32 and a fixed
+ * order.  ids [T, topk] int64 or int32 (ids outside [0, E) contribute nothing), weights [T, topk] of weight_dtype;
+ * w13 [E, 2f, d], w2 [E, d, f] and their scales as exl3_fp8_mlp, per expert.  topk <= 32. */
+EXL3_API int64_t exl3_fp8_experts_workspace(int64_t T, int64_t topk, int64_t E, int64_t d, int64_t f);
+EXL3_API int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_stride, const void* ids,
+                              int ids_is_int64, const void* weights, int64_t weight_dtype, int64_t topk, int64_t E,
+                              const void* w13, const float* w13_scale, const void* w2, const float* w2_scale,
+                              int64_t f, double limit, void* out, int64_t out_dtype, int64_t out_stride,
+                              int accumulate, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Expert parallelism.  No reference counterpart: the reference refuses expert-parallel layers
