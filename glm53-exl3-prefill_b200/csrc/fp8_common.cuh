@@ -80,7 +80,7 @@ __device__ __forceinline__ float clamped_swiglu(float g, float u, float limit)
 {
     g = g > limit ? limit : g;
     u = u > limit ? limit : (u < -limit ? -limit : u);
-    return g / (1.0f + expf(-g)) * u;
+    return __fdividef(g, 1.0f + __expf(-g)) * u;
 }
 
 }  // namespace fp8
