@@ -12,21 +12,23 @@
 // accumulation in TMEM (four tcgen05.mma of K = 32, fp32), which epilogue warps take out, scale and add to
 // fp32 sums in registers while the tensor core works on the next block in the other TMEM buffer.
 //
-// A tile is up to 128 rows (tokens) by 256 weight rows (two blocks of 128: neighbours, or the gate and up rows of
-// the same columns for swiglu), in one of two orientations:
-//   wide  (more than FG_THIN rows)  tokens are the MMA's M: TMEM lane = token, column = weight row.  The scale
-//         is one register per thread, so the epilogue reads next to nothing from shared memory;
-//   thin  weights are M: lane = weight row, column = token, N = the tile's rows rounded up to 16, so an
-//         expert with few rows costs few columns.  Here every value needs its column's scale, which a warp reads from
-//         shared memory (128 bytes a clock for the SM, operands of the MMA included): 8 clocks per column and
-//         K block, 1024 for 128 columns, where the MMA takes 512.  Up to 64 columns it is the cheaper form.
+// Two CTAs (a cluster) work on one tile with cta_group::2 MMAs, M = 256 over the pair: a single SM's operands
+// (A and B of 128 x 256 x 32: 12 KB per 128 clocks at the full rate, beside 48 KB of new data per K block) come out of
+// shared memory at two thirds of the tensor core's rate; the pair holds each operand once between two SMs.
+// A tile is a run of rows (tokens) of one expert by 256 or 512 weight rows, in one of two orientations:
+//   wide  (129..256 rows)  tokens are M: CTA r holds tokens 128 r .. 128 r + 127 and weight block r of two (neighbours,
+//         or the gate and up rows of the same columns for swiglu); TMEM lane = token, column = weight row of
+//         both blocks.  The scale is one register per thread.
+//   thin  (up to 128 rows)  weights are M: CTA r holds two weight blocks of four (for swiglu gate and up of its own
+//         128 columns) and half of the tokens, N = the tile's rows rounded up to 16; lane = weight row, column =
+//         token.  An expert with few rows costs few columns.  Every value needs its column's scale here, which a warp
+//         reads from shared memory (128 bytes a clock for the SM): 8 clocks per column and K block.
 //
-//   warp 0        TMA producer: weight blocks [128 x 128 B] x 2 and token rows in boxes of 32, 128-byte swizzle;
-//   warp 1        MMA issuer, TMEM owner;
-//   warps 2, 3    scales: sx * sw of the coming K blocks into a shared-memory ring, loaded one group ahead;
-//   warps 4..11   two warpgroups of epilogue: warpgroup g takes 64 columns of each block (wide), or every other
-//                 chunk of 16 columns (thin).
-// Persistent CTAs walk the tiles (expert, weight tile, token tile; token tiles fastest, so the CTAs running at
+//   warp 0        TMA producer of this CTA's operands: weight blocks [128 x 128 B], token rows in boxes of 32;
+//   warp 1        MMA issuer (in CTA 0, for both), TMEM owner;
+//   warps 2, 3    scales of the coming K blocks into a shared-memory ring (cp.async, up to eight blocks ahead);
+//   warps 4..19   four warpgroups of epilogue: warpgroup g takes 32 columns of each block (wide) or 32 tokens (thin).
+// The clusters walk the tiles (expert, weight tile, token tile; token tiles fastest, so the clusters running at
 // one time share weight tiles through L2).  Every wait is bounded as in the trellis kernels.
 #include <cuda.h>
 
@@ -39,25 +41,27 @@ namespace {
 
 using namespace fp8;
 
-constexpr int FG_THREADS = 384;
+constexpr int FG_EPI_WARPS = 16;
+constexpr int FG_EPI_THREADS = FG_EPI_WARPS * 32;
+constexpr int FG_THREADS = 128 + FG_EPI_THREADS;
 constexpr int FG_BK = 128;                                  // K bytes per stage: one 128-byte swizzle atom
 constexpr uint32_t FG_W_BYTES = 128 * FG_BK;                // one block of weight rows
 constexpr int FG_XBOX = 32;                                 // token rows per TMA box
-constexpr int NT = 128;                                     // token rows of a tile
-constexpr int FG_THIN = 64;                                 // most rows of a thin tile
-constexpr int FG_STAGES = 4;
-constexpr uint32_t FG_STAGE_BYTES = 2 * FG_W_BYTES + NT * FG_BK;
+constexpr int NT = 128;                                     // tokens of a CTA in a wide tile, of the pair in a thin one
+constexpr int FG_STAGES = 5;
+constexpr uint32_t FG_STAGE_BYTES = 2 * FG_W_BYTES + 64 * FG_BK;    // thin: two weight blocks, 64 tokens
 constexpr int FG_SCALES = 8;                                // slots of the scale ring
 constexpr uint64_t FG_DRAIN_NS = 200000000ull;
 
 struct Fp8GemmArgs {
     int N, K, n_experts;
-    int n_tiles_n, num_kb;
+    int n_wide, n_thin, num_kb;      // weight tiles of a wide and of a thin row tile; K blocks
+    int n_blocks;                    // weight blocks of 128 rows
     int single_count;                // rows of the one expert when counts is null
     const int32_t* counts;           // [E] or null
     const int32_t* row0;             // [E] first row of each expert, or null
     const float* sx; int64_t sx_row, sx_blk;
-    const float* sw; int64_t sw_expert, sw_n, sw_k;
+    const float* sw; int64_t sw_expert, sw_n;
     // store
     void* out; int64_t out_stride; int out_dtype; int accumulate;
     int out_vec;                     // rows are 16-byte aligned
@@ -69,14 +73,57 @@ struct Fp8GemmArgs {
     uint64_t wait_ns;
 };
 
-__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate)
+// D (both CTAs' TMEM) (+)= A . B^T over the pair: M = 256, each CTA holding 128 rows of A and N / 2 rows of B.
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate)
 {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Arrive (once) on `bar` in the CTAs of `mask` when every MMA issued so far by this thread has completed.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint16_t mask = 3)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 :: "r"(smem_u32(bar)), "h"(mask) : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// The address of `p` in CTA 0 of the cluster.
+__device__ __forceinline__ uint32_t in_cta0(const void* p)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+
+// One lane of a converged warp.  Roles of a single thread run as a whole warp with the instruction itself behind this:
+// with the loop inside an `if (lane == 0)` the compiler cannot keep descriptors and addresses in uniform
+// registers, and the MMA thread took 1300 clocks per K block.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 
 // Instruction descriptor, kind::f8f6f4: D fp32, A and B e4m3 (both K-major), shape M x N.
@@ -85,44 +132,66 @@ __device__ __forceinline__ uint32_t idesc_e4m3_f32(int M, int N)
     return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, int32_t x, int32_t y, int32_t z,
-                                            uint64_t* bar)
+// Tiled loads into this CTA's shared memory that complete on a barrier (`bar`) of CTA 0.
+__device__ __forceinline__ void tma_pair_3d(void* smem_dst, const void* tmap, int32_t x, int32_t y, int32_t z, uint32_t bar)
 {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        :: "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];"
+        :: "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 
-// 32 (16) consecutive columns of this warp's 32 TMEM lanes as register pairs, complete on return.
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint64_t (&d)[16])
+__device__ __forceinline__ void tma_pair_2d(void* smem_dst, const void* tmap, int32_t x, int32_t y, uint32_t bar)
 {
     asm volatile(
-        "{\n\t.reg .b32 t<32>;\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, t11, t12, t13, t14, t15, t16, t17, t18, t19, t20, t21, t22, t23, t24, t25, t26, t27, t28, t29, t30, t31}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;\n\t"
-        "mov.b64 %0, {t0, t1};\n\t"
-        "mov.b64 %1, {t2, t3};\n\t"
-        "mov.b64 %2, {t4, t5};\n\t"
-        "mov.b64 %3, {t6, t7};\n\t"
-        "mov.b64 %4, {t8, t9};\n\t"
-        "mov.b64 %5, {t10, t11};\n\t"
-        "mov.b64 %6, {t12, t13};\n\t"
-        "mov.b64 %7, {t14, t15};\n\t"
-        "mov.b64 %8, {t16, t17};\n\t"
-        "mov.b64 %9, {t18, t19};\n\t"
-        "mov.b64 %10, {t20, t21};\n\t"
-        "mov.b64 %11, {t22, t23};\n\t"
-        "mov.b64 %12, {t24, t25};\n\t"
-        "mov.b64 %13, {t26, t27};\n\t"
-        "mov.b64 %14, {t28, t29};\n\t"
-        "mov.b64 %15, {t30, t31};\n\t"
-        "}"
-        : "=l"(d[0]), "=l"(d[1]), "=l"(d[2]), "=l"(d[3]), "=l"(d[4]), "=l"(d[5]), "=l"(d[6]), "=l"(d[7]), "=l"(d[8]), "=l"(d[9]), "=l"(d[10]), "=l"(d[11]), "=l"(d[12]), "=l"(d[13]), "=l"(d[14]), "=l"(d[15])
-        : "r"(taddr));
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];"
+        :: "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_dst, uint32_t ncols)
+{
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(smem_dst)), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols)
+{
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(taddr), "r"(ncols) : "memory");
+}
+
+__device__ __forceinline__ void cp_async4(void* smem_dst, const void* gmem_src)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(smem_u32(smem_dst)), "l"(gmem_src) : "memory");
+}
+
+// Arrive (once per thread) on `bar` when this thread's cp.async copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void cp_async_wait_all()
+{
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Non-blocking test of one phase each of two barriers.
+__device__ __forceinline__ bool mbar_test_wait2(uint64_t* bar_a, uint32_t parity_a, uint64_t* bar_b, uint32_t parity_b)
+{
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred pa, pb;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 pa, [%1], %2;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 pb, [%3], %4;\n\t"
+        "and.pred pa, pa, pb;\n\t"
+        "selp.u32 %0, 1, 0, pa;\n\t}"
+        : "=r"(done) : "r"(smem_u32(bar_a)), "r"(parity_a), "r"(smem_u32(bar_b)), "r"(parity_b) : "memory");
+    return done != 0;
+}
+
+// 16 consecutive columns of this warp's 32 TMEM lanes as register pairs, complete on return.
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint64_t (&d)[8])
 {
     asm volatile(
@@ -164,36 +233,83 @@ __device__ __forceinline__ void fma2(uint64_t& a, uint64_t d, uint64_t s)
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(d), "l"(s));
 }
 
-struct Tile {
-    bool thin;
-    int e, nt, row0, rows, nh;       // nh: weight blocks with rows (1 at the end of an odd number of blocks)
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// mbar_wait by a whole warp, with one answer for it.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                          uint64_t limit_ns)
+{
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, limit_ns));
+}
+
+// Position in a ring of N barriers: slot and the parity of the current pass.
+template <int N>
+struct Ring {
+    int slot = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next()
+    {
+        if (++slot == N)
+        {
+            slot = 0;
+            parity ^= 1u;
+        }
+    }
 };
 
-template <bool SWIGLU>
+struct Tile {
+    bool thin;
+    int e, nt;
+    int row0, rows;                  // rows of the tile (of both CTAs)
+    int ncols;                       // thin: rows rounded up to 16
+};
+
+// 256-row tiles of an expert with `count` rows, and whether its last rows (up to 128) are a thin tile.
+__device__ __forceinline__ int wide_tiles(int count) { return count / 256 + (count % 256 > 128 ? 1 : 0); }
+__device__ __forceinline__ int thin_tiles(int count) { const int r = count % 256; return r > 0 && r <= 128 ? 1 : 0; }
+
+__device__ __forceinline__ int row_count(const Fp8GemmArgs& p, int e)
+{
+    return p.counts ? __ldg(p.counts + e) : p.single_count;
+}
+
+__device__ __forceinline__ int expert_tiles(const Fp8GemmArgs& p, int e)
+{
+    const int count = row_count(p, e);
+    return wide_tiles(count) * p.n_wide + thin_tiles(count) * p.n_thin;
+}
+
 __device__ __forceinline__ Tile tile_at(const Fp8GemmArgs& p, const int* pref, int t)
 {
     Tile ti;
-    ti.e = trellis::prefix_find(pref, p.n_experts, t / p.n_tiles_n);
-    const int mts = pref[ti.e + 1] - pref[ti.e];
-    const int local = t - pref[ti.e] * p.n_tiles_n;
-    ti.nt = local / mts;
-    const int mt = local - ti.nt * mts;
-    const int count = p.counts ? __ldg(p.counts + ti.e) : p.single_count;
-    ti.row0 = (p.row0 ? __ldg(p.row0 + ti.e) : 0) + mt * NT;
-    ti.rows = min(NT, count - mt * NT);
-    ti.thin = ti.rows <= FG_THIN;
-    ti.nh = SWIGLU || ti.nt * 256 + 128 < p.N ? 2 : 1;
+    ti.e = trellis::prefix_find(pref, p.n_experts, t);
+    const int count = row_count(p, ti.e), wide = wide_tiles(count);
+    const int local = t - pref[ti.e];
+    ti.thin = local >= wide * p.n_wide;
+    ti.nt = ti.thin ? local - wide * p.n_wide : local / wide;
+    const int first = ti.thin ? count / 256 * 256 : (local - ti.nt * wide) * 256;
+    ti.row0 = (p.row0 ? __ldg(p.row0 + ti.e) : 0) + first;
+    ti.rows = min(256, count - first);
+    ti.ncols = (ti.rows + 15) & ~15;
     return ti;
 }
 
-// Weight block (of 128 rows) that is half h of tile column nt.
+// Weight block (of 128 rows) h (0, 1) of CTA r: wide tiles have one per CTA (h = r, whatever is asked for the epilogue),
+// thin ones two.  May be past the last block: loads there give zeros.
 template <bool SWIGLU>
-__device__ __forceinline__ int weight_block(const Fp8GemmArgs& p, int nt, int h)
+__device__ __forceinline__ int weight_block(const Fp8GemmArgs& p, const Tile& ti, int r, int h)
 {
-    return SWIGLU ? h * (p.f / kBlock) + nt : 2 * nt + h;
+    if (!ti.thin) return SWIGLU ? h * (p.f / kBlock) + ti.nt : 2 * ti.nt + h;
+    return SWIGLU ? h * (p.f / kBlock) + 2 * ti.nt + r : 4 * ti.nt + 2 * r + h;
 }
 
-constexpr int FG_STEP = 8;                                  // tokens staged at a time by a warpgroup
+constexpr int FG_STEP = 4;                                  // tokens staged at a time by a warpgroup
 
 // Eight consecutive outputs of one row.
 template <class To>
@@ -217,64 +333,48 @@ __device__ __forceinline__ void store8(const Fp8GemmArgs& p, int64_t r, int n, c
         if (n + i < p.N) o[i] = from_float<To>(p.accumulate ? to_float(o[i]) + a[i] : a[i]);
 }
 
-// Thin tiles: the staged tokens [m0, m0 + FG_STEP) x 256 weight rows, by the 128 threads of a warpgroup.
+// Thin tiles: the staged tokens [m0, m0 + FG_STEP) x 256 weight rows of CTA r, by the 128 threads of a warpgroup.
 template <bool SWIGLU>
-__device__ __forceinline__ void write_step(const Fp8GemmArgs& p, const Tile& ti, const float* st, int m0, int tid)
+__device__ __forceinline__ void write_step(const Fp8GemmArgs& p, const Tile& ti, int r0, const float* st, int m0, int tid)
 {
     if constexpr (!SWIGLU)
     {
-        #pragma unroll 1
-        for (int u = tid; u < FG_STEP * 32; u += 128)
-        {
-            const int m = m0 + (u >> 5), c = (u & 31) * 8, n = ti.nt * 256 + c;
-            if (m >= ti.rows || n >= p.N) continue;
-            const int64_t r = p.slot ? __ldg(p.slot + ti.row0 + m) : (int64_t) ti.row0 + m;
-            const float* v = st + (u >> 5) * 256 + c;
-            if (p.out_dtype == 0) store8<float>(p, r, n, v);
-            else if (p.out_dtype == 1) store8<__half>(p, r, n, v);
-            else store8<__nv_bfloat16>(p, r, n, v);
-        }
+        const int m = m0 + (tid >> 5), c = (tid & 31) * 8, n = (2 * ti.nt + r0) * 256 + c;
+        if (m >= ti.rows || n >= p.N) return;
+        const int64_t r = p.slot ? __ldg(p.slot + ti.row0 + m) : (int64_t) ti.row0 + m;
+        const float* v = st + (tid >> 5) * 256 + c;
+        if (p.out_dtype == 0) store8<float>(p, r, n, v);
+        else if (p.out_dtype == 1) store8<__half>(p, r, n, v);
+        else store8<__nv_bfloat16>(p, r, n, v);
     }
     else
     {
-        // 16 lanes per token, 8 columns each; the block's largest magnitude is four shuffles
-        const int m = m0 + (tid >> 4), c = tid & 15;
-        const float* v = st + (tid >> 4) * 256 + c * 4;
-        float a[8];
+        // a warp per token, 4 columns a lane
+        const int m = m0 + (tid >> 5), c = tid & 31;
+        const float4 g = *reinterpret_cast<const float4*>(st + (tid >> 5) * 256 + c * 4);
+        const float4 u = *reinterpret_cast<const float4*>(st + (tid >> 5) * 256 + 128 + c * 4);
+        const float a[4] = {clamped_swiglu(g.x, u.x, p.limit), clamped_swiglu(g.y, u.y, p.limit),
+                            clamped_swiglu(g.z, u.z, p.limit), clamped_swiglu(g.w, u.w, p.limit)};
         uint32_t mx = 0;
         #pragma unroll
-        for (int i = 0; i < 2; ++i)
-        {
-            const float4 g = *reinterpret_cast<const float4*>(v + 64 * i);
-            const float4 u = *reinterpret_cast<const float4*>(v + 64 * i + 128);
-            a[4 * i] = clamped_swiglu(g.x, u.x, p.limit);
-            a[4 * i + 1] = clamped_swiglu(g.y, u.y, p.limit);
-            a[4 * i + 2] = clamped_swiglu(g.z, u.z, p.limit);
-            a[4 * i + 3] = clamped_swiglu(g.w, u.w, p.limit);
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) mx = max(mx, __float_as_uint(a[4 * i + j]) & 0x7fffffffu);
-        }
-        #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (m >= ti.rows) return;
+        for (int j = 0; j < 4; ++j) mx = max(mx, __float_as_uint(a[j]) & 0x7fffffffu);
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        const int fb = 2 * ti.nt + r0;
+        if (m >= ti.rows || fb * kBlock >= p.f) return;
         const float s = block_scale(__uint_as_float(mx), false), inv = 1.0f / s;
         const int64_t r = ti.row0 + m;
-        uint32_t* h = reinterpret_cast<uint32_t*>(p.h + r * p.h_stride + ti.nt * kBlock) + c;
+        float q[4];
         #pragma unroll
-        for (int i = 0; i < 2; ++i)
-        {
-            float q[4];
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = quotient(a[4 * i + j], s, inv);
-            h[16 * i] = to_e4m3x2(q[0], q[1]) | to_e4m3x2(q[2], q[3]) << 16;
-        }
-        if (c == 0) p.hs[r * p.hs_row + ti.nt * p.hs_blk] = s;
+        for (int j = 0; j < 4; ++j) q[j] = quotient(a[j], s, inv);
+        reinterpret_cast<uint32_t*>(p.h + r * p.h_stride + fb * kBlock)[c] =
+            to_e4m3x2(q[0], q[1]) | to_e4m3x2(q[2], q[3]) << 16;
+        if (c == 0) p.hs[r * p.hs_row + fb * p.hs_blk] = s;
     }
 }
 
-// Wide tiles, store: this thread's token, 64 columns of each of the two weight blocks.
+// Wide tiles, store: this thread's token, 32 columns of each of the two weight blocks.
 template <class To>
-__device__ __forceinline__ void store_wide(const Fp8GemmArgs& p, const Tile& ti, const uint64_t (&acc)[2][32], int g, int m)
+__device__ __forceinline__ void store_wide(const Fp8GemmArgs& p, const Tile& ti, const uint64_t (&acc)[2][16], int g, int m)
 {
     if (m >= ti.rows) return;
     const int64_t r = p.slot ? __ldg(p.slot + ti.row0 + m) : (int64_t) ti.row0 + m;
@@ -283,11 +383,11 @@ __device__ __forceinline__ void store_wide(const Fp8GemmArgs& p, const Tile& ti,
     #pragma unroll
     for (int h = 0; h < 2; ++h)
     {
-        const int n0 = ti.nt * 256 + h * 128 + g * 64;
-        if (p.out_vec && !p.accumulate && n0 + 64 <= p.N)
+        const int n0 = ti.nt * 256 + h * 128 + g * 32;
+        if (p.out_vec && !p.accumulate && n0 + 32 <= p.N)
         {
             #pragma unroll
-            for (int c = 0; c < 64; c += PER)
+            for (int c = 0; c < 32; c += PER)
             {
                 __align__(16) To w[PER];
                 #pragma unroll
@@ -301,7 +401,7 @@ __device__ __forceinline__ void store_wide(const Fp8GemmArgs& p, const Tile& ti,
         else
         {
             #pragma unroll
-            for (int c = 0; c < 64; ++c)
+            for (int c = 0; c < 32; ++c)
                 if (n0 + c < p.N)
                 {
                     float v = half_of(acc[h][c >> 1], c & 1);
@@ -313,32 +413,33 @@ __device__ __forceinline__ void store_wide(const Fp8GemmArgs& p, const Tile& ti,
 }
 
 template <bool SWIGLU>
-__global__ __launch_bounds__(FG_THREADS, 1)
+__global__ __cluster_dims__(2, 1, 1) __launch_bounds__(FG_THREADS, 1)
 void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                      const Fp8GemmArgs p)
 {
     constexpr uint32_t TMEM_COLS = 512;                     // two buffers of 256 columns
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bar_full[FG_STAGES], bar_empty[FG_STAGES];
+    __shared__ uint64_t bar_full[FG_STAGES];                // CTA 0: both CTAs' operands of a stage have landed
+    __shared__ uint64_t bar_done[FG_STAGES];                // its MMAs are done: the stage is free, the sums are in TMEM
     __shared__ uint64_t bar_sfull[FG_SCALES], bar_sempty[FG_SCALES];
-    __shared__ uint64_t bar_tfull[2], bar_tempty[2], bar_done;
+    __shared__ uint64_t bar_tempty[2];                      // CTA 0: both CTAs have taken a TMEM buffer's sums out
+    __shared__ __align__(16) float s_sx[FG_SCALES][NT];
+    __shared__ float s_sw[FG_SCALES][2];
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort, s_fail;
     __shared__ int s_pref[kMaxExperts + 1];
-    __shared__ __align__(16) float s_scale[FG_SCALES][2][NT];
-    __shared__ __align__(16) float s_stage[2][FG_STEP][256];
-    __shared__ uint32_t s_amax[2][NT];
+    __shared__ __align__(16) float s_stage[4][FG_STEP][256];
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int) cluster_rank();
+    const int cluster = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
 
     if (warp == 0)
     {
-        // tiles of rows per expert, as an exclusive prefix
+        // tiles per expert, as an exclusive prefix
         const int per = (p.n_experts + 31) / 32;
-        auto tiles = [&](int e) {
-            return e < p.n_experts ? ((p.counts ? __ldg(p.counts + e) : p.single_count) + NT - 1) / NT : 0;
-        };
+        auto tiles = [&](int e) { return e < p.n_experts ? expert_tiles(p, e) : 0; };
         int sum = 0;
         for (int i = 0; i < per; ++i) sum += tiles(lane * per + i);
         int inc = sum;
@@ -364,251 +465,223 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             for (int s = 0; s < FG_STAGES; ++s)
             {
                 mbar_init(&bar_full[s], 1);
-                mbar_init(&bar_empty[s], 1);
+                mbar_init(&bar_done[s], 1);
             }
             for (int s = 0; s < FG_SCALES; ++s)
             {
-                mbar_init(&bar_sfull[s], 2);
-                mbar_init(&bar_sempty[s], 8);
+                mbar_init(&bar_sfull[s], 64);
+                mbar_init(&bar_sempty[s], FG_EPI_WARPS);
             }
-            for (int b = 0; b < 2; ++b)
-            {
-                mbar_init(&bar_tfull[b], 1);
-                mbar_init(&bar_tempty[b], 8);
-            }
-            mbar_init(&bar_done, 1);
+            for (int b = 0; b < 2; ++b) mbar_init(&bar_tempty[b], 2 * FG_EPI_WARPS);
             s_abort = 0;
             s_fail = 0;
             fence_mbar_init();
         }
         __syncwarp();
-        tmem_alloc(&s_tmem_base, TMEM_COLS);
-        tmem_relinquish();
+        tmem_alloc_pair(&s_tmem_base, TMEM_COLS);
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync();                                         // both CTAs' barriers and TMEM exist
     tc_fence_after();
     const uint32_t tmem_base = s_tmem_base;
     volatile int* abort_flag = &s_abort;
-    const int total = s_pref[p.n_experts] * p.n_tiles_n;
+    const int total = s_pref[p.n_experts];
     const int nkb = p.num_kb;
 
     if (warp < 4)
     {
-        setmaxnreg_dec<88>();
+        setmaxnreg_dec<56>();
         if (warp == 0)
         {
             // ============================================================ TMA producer
-            if (lane == 0)
+            Ring<FG_STAGES> st;
+            int issued = 0;
+            bool ok = true;
+            for (int t = cluster; ok && t < total; t += n_clusters)
             {
-                int issued = 0;
-                bool ok = true;
-                for (int t = blockIdx.x; ok && t < total; t += gridDim.x)
+                const Tile ti = tile_at(p, s_pref, t);
+                // boxes of CTA r and the pair's bytes: wide, one weight block and up to 128 tokens a CTA; thin, two
+                // weight blocks and half of the columns
+                const int half = ti.ncols / 2;
+                const int boxes0 = ti.thin ? (half + FG_XBOX - 1) / FG_XBOX : 4;
+                const int boxes1 = ti.thin ? boxes0 : (ti.rows - 128 + FG_XBOX - 1) / FG_XBOX;
+                const uint32_t bytes = (ti.thin ? 4 : 2) * FG_W_BYTES + (boxes0 + boxes1) * (FG_XBOX * FG_BK);
+                const int boxes = rank ? boxes1 : boxes0;
+                const int row = ti.row0 + rank * (ti.thin ? half : 128);
+                const int w_row0 = weight_block<SWIGLU>(p, ti, rank, ti.thin ? 0 : rank) * kBlock;
+                const int w_row1 = weight_block<SWIGLU>(p, ti, rank, 1) * kBlock;
+                const uint32_t x_off = ti.thin ? 2 * FG_W_BYTES : FG_W_BYTES;
+                for (int kb = 0; kb < nkb; ++kb, ++issued, st.next())
                 {
-                    const Tile ti = tile_at<SWIGLU>(p, s_pref, t);
-                    const int boxes = (ti.rows + FG_XBOX - 1) / FG_XBOX;
-                    const uint32_t bytes = ti.nh * FG_W_BYTES + boxes * (FG_XBOX * FG_BK);
-                    for (int kb = 0; kb < nkb; ++kb, ++issued)
+                    // (the first pass does not wait: a fresh barrier counts as past the phase of parity 1)
+                    ok = warp_wait(&bar_done[st.slot], st.parity ^ 1u, abort_flag, p.status, p.wait_ns);
+                    if (!ok) break;
+                    if (elect_one())
                     {
-                        const int s = issued % FG_STAGES;
-                        const uint32_t ph = (issued / FG_STAGES) & 1u;
-                        if (issued >= FG_STAGES && !mbar_wait(&bar_empty[s], ph ^ 1u, abort_flag, p.status, p.wait_ns))
-                        {
-                            ok = false;
-                            break;
-                        }
-                        uint8_t* w = smem + s * FG_STAGE_BYTES;
-                        mbar_arrive_expect_tx(&bar_full[s], bytes);
-                        for (int h = 0; h < ti.nh; ++h)
-                            tma_load_3d(w + h * FG_W_BYTES, &tmap_w, kb * FG_BK, weight_block<SWIGLU>(p, ti.nt, h) * kBlock,
-                                        ti.e, &bar_full[s]);
+                        uint8_t* w = smem + st.slot * FG_STAGE_BYTES;
+                        const uint32_t full = in_cta0(&bar_full[st.slot]);
+                        if (rank == 0) mbar_arrive_expect_tx(&bar_full[st.slot], bytes);
+                        tma_pair_3d(w, &tmap_w, kb * FG_BK, w_row0, ti.e, full);
+                        if (ti.thin) tma_pair_3d(w + FG_W_BYTES, &tmap_w, kb * FG_BK, w_row1, ti.e, full);
                         for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(w + 2 * FG_W_BYTES + b * (FG_XBOX * FG_BK), &tmap_x, kb * FG_BK,
-                                        ti.row0 + b * FG_XBOX, &bar_full[s]);
+                            tma_pair_2d(w + x_off + b * (FG_XBOX * FG_BK), &tmap_x, kb * FG_BK, row + b * FG_XBOX, full);
                     }
+                    __syncwarp();
                 }
-                // copies in flight land before the CTA's shared memory goes away
-                for (int i = issued > FG_STAGES ? issued - FG_STAGES : 0; i < issued; ++i)
-                    mbar_drain(&bar_full[i % FG_STAGES], (i / FG_STAGES) & 1u, FG_DRAIN_NS);
             }
+            // a stage whose MMAs are done has landed; after an abort this gives the copies in flight their time
+            for (int i = issued > FG_STAGES ? issued - FG_STAGES : 0; i < issued; ++i)
+                mbar_drain(&bar_done[i % FG_STAGES], (i / FG_STAGES) & 1u, FG_DRAIN_NS);
         }
         else if (warp == 1)
         {
             // ============================================================ MMA issuer
-            if (lane == 0)
+            if (rank == 0)
             {
-                int it = 0;
+                Ring<FG_STAGES> st;
+                Ring<2> buf;
                 bool ok = true;
-                for (int t = blockIdx.x; ok && t < total; t += gridDim.x)
+                for (int t = cluster; ok && t < total; t += n_clusters)
                 {
-                    const Tile ti = tile_at<SWIGLU>(p, s_pref, t);
-                    const uint32_t idesc = idesc_e4m3_f32(128, ti.thin ? (ti.rows + 15) & ~15 : ti.nh * 128);
-                    for (int kb = 0; kb < nkb; ++kb, ++it)
+                    const Tile ti = tile_at(p, s_pref, t);
+                    const uint32_t idesc = idesc_e4m3_f32(256, ti.thin ? ti.ncols : 256);
+                    for (int kb = 0; kb < nkb; ++kb, st.next(), buf.next())
                     {
-                        const int s = it % FG_STAGES, b = it & 1;
-                        if ((it >= 2 && !mbar_wait(&bar_tempty[b], ((it >> 1) & 1u) ^ 1u, abort_flag, p.status, p.wait_ns)) ||
-                            !mbar_wait(&bar_full[s], (it / FG_STAGES) & 1u, abort_flag, p.status, p.wait_ns))
-                        {
-                            ok = false;
-                            break;
-                        }
+                        ok = warp_wait(&bar_tempty[buf.slot], buf.parity ^ 1u, abort_flag, p.status, p.wait_ns) &&
+                             warp_wait(&bar_full[st.slot], st.parity, abort_flag, p.status, p.wait_ns);
+                        if (!ok) break;
                         tc_fence_after();
-                        const uint32_t w = smem_u32(smem + s * FG_STAGE_BYTES);
-                        const uint64_t x_desc = smem_desc_sw128(w + 2 * FG_W_BYTES), w_desc = smem_desc_sw128(w);
-                        const uint32_t d = tmem_base + b * 256;
-                        if (ti.thin)
+                        const uint32_t w = smem_u32(smem) + st.slot * FG_STAGE_BYTES;
+                        const uint64_t w_desc = smem_desc_sw128(w);
+                        const uint32_t d = tmem_base + buf.slot * 256;
+                        if (elect_one())
                         {
-                            for (int h = 0; h < ti.nh; ++h)
+                            if (ti.thin)
+                            {
+                                const uint64_t x_desc = w_desc + (2 * FG_W_BYTES >> 4);
+                                #pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    #pragma unroll
+                                    for (int kk = 0; kk < FG_BK / 32; ++kk)
+                                        umma_e4m3_pair(d + h * 128, w_desc + h * (FG_W_BYTES >> 4) + 2 * kk,
+                                                       x_desc + 2 * kk, idesc, kk != 0);
+                            }
+                            else
+                            {
+                                const uint64_t x_desc = w_desc + (FG_W_BYTES >> 4);
                                 #pragma unroll
                                 for (int kk = 0; kk < FG_BK / 32; ++kk)
-                                    umma_e4m3(d + h * 128, w_desc + h * (FG_W_BYTES >> 4) + 2 * kk, x_desc + 2 * kk, idesc, kk != 0);
+                                    umma_e4m3_pair(d, x_desc + 2 * kk, w_desc + 2 * kk, idesc, kk != 0);
+                            }
+                            umma_commit_pair(&bar_done[st.slot]);
                         }
-                        else
-                        {
-                            #pragma unroll
-                            for (int kk = 0; kk < FG_BK / 32; ++kk)
-                                umma_e4m3(d, x_desc + 2 * kk, w_desc + 2 * kk, idesc, kk != 0);
-                        }
-                        umma_commit(&bar_empty[s]);
-                        umma_commit(&bar_tfull[b]);
+                        __syncwarp();
                     }
                 }
-                umma_commit(&bar_done);
-                mbar_drain(&bar_done, 0, FG_DRAIN_NS);
+                // the MMAs of the last stages are done before the CTAs leave: the producer's drain waits for them
             }
         }
         else
         {
             // ============================================================ scales
-            constexpr int PER = NT >= 64 ? NT / 64 : 1;     // columns per lane
-            constexpr int AHEAD = 4;                        // K blocks loaded together
-            const int j0 = (warp - 2) * 32 + lane;
-            int it = 0;
+            const int j = (warp - 2) * 32 + lane;           // tokens j and j + 64; weight block j for j < 2
+            Ring<FG_SCALES> sr;
             bool ok = true;
-            for (int t = blockIdx.x; ok && t < total; t += gridDim.x)
+            for (int t = cluster; ok && t < total; t += n_clusters)
             {
-                const Tile ti = tile_at<SWIGLU>(p, s_pref, t);
-                const float* sw0 = p.sw + ti.e * p.sw_expert + weight_block<SWIGLU>(p, ti.nt, 0) * p.sw_n;
-                const float* sw1 = ti.nh > 1 ? p.sw + ti.e * p.sw_expert + weight_block<SWIGLU>(p, ti.nt, 1) * p.sw_n : sw0;
-                float x[PER][AHEAD], w0[AHEAD], w1[AHEAD];
-                auto load = [&](int kb0) {
-                    #pragma unroll
-                    for (int a = 0; a < AHEAD; ++a)
-                    {
-                        const bool in = kb0 + a < nkb;
-                        w0[a] = in ? __ldg(sw0 + (kb0 + a) * p.sw_k) : 0.0f;
-                        w1[a] = in ? __ldg(sw1 + (kb0 + a) * p.sw_k) : 0.0f;
-                        #pragma unroll
-                        for (int i = 0; i < PER; ++i)
-                        {
-                            const int m = j0 + 64 * i;
-                            x[i][a] = in && m < ti.rows ? __ldg(p.sx + (ti.row0 + m) * p.sx_row + (kb0 + a) * p.sx_blk) : 0.0f;
-                        }
-                    }
-                };
-                load(0);
-                for (int kb0 = 0; ok && kb0 < nkb; kb0 += AHEAD)
+                const Tile ti = tile_at(p, s_pref, t);
+                const int rows = ti.thin ? ti.rows : min(128, ti.rows - 128 * rank);
+                const float* sx = p.sx + (int64_t) (ti.row0 + (ti.thin ? 0 : 128 * rank) + j) * p.sx_row;
+                // a block past the last one has sums of zero: any scale will do
+                const float* sw = p.sw + ti.e * p.sw_expert + min(weight_block<SWIGLU>(p, ti, rank, j & 1), p.n_blocks - 1) * p.sw_n;
+                for (int kb = 0; kb < nkb; ++kb, sr.next())
                 {
-                    float o0[PER][AHEAD], o1[PER][AHEAD];
-                    #pragma unroll
-                    for (int a = 0; a < AHEAD; ++a)
-                        #pragma unroll
-                        for (int i = 0; i < PER; ++i)
-                        {
-                            o0[i][a] = x[i][a] * w0[a];
-                            o1[i][a] = x[i][a] * w1[a];
-                        }
-                    if (kb0 + AHEAD < nkb) load(kb0 + AHEAD);
-                    #pragma unroll
-                    for (int a = 0; a < AHEAD; ++a)
-                    {
-                        if (kb0 + a >= nkb) break;
-                        const int q = it % FG_SCALES;
-                        if (it >= FG_SCALES &&
-                            !__all_sync(0xffffffffu, mbar_wait(&bar_sempty[q], ((it / FG_SCALES) & 1u) ^ 1u, abort_flag,
-                                                               p.status, p.wait_ns)))
-                        {
-                            ok = false;
-                            break;
-                        }
-                        #pragma unroll
-                        for (int i = 0; i < PER; ++i)
-                            if (j0 + 64 * i < NT)
-                            {
-                                s_scale[q][0][j0 + 64 * i] = o0[i][a];
-                                s_scale[q][1][j0 + 64 * i] = o1[i][a];
-                            }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bar_sfull[q]);
-                        ++it;
-                    }
+                    const int q = sr.slot;
+                    ok = warp_wait(&bar_sempty[q], sr.parity ^ 1u, abort_flag, p.status, p.wait_ns);
+                    if (!ok) break;
+                    if (j < rows) cp_async4(&s_sx[q][j], sx);
+                    if (j + 64 < rows) cp_async4(&s_sx[q][j + 64], sx + 64 * p.sx_row);
+                    if (j < 2) cp_async4(&s_sw[q][j], sw);
+                    cp_async_arrive(&bar_sfull[q]);
+                    sx += p.sx_blk;
+                    sw += 1;
                 }
             }
+            cp_async_wait_all();
         }
     }
     else
     {
         // ================================================================ epilogue
-        setmaxnreg_inc<208>();
+        setmaxnreg_inc<104>();
         const int g = (warp - 4) >> 2;                      // warpgroup
         const int quarter = warp & 3;
         const int lane_in = quarter * 32 + lane;            // TMEM lane: token (wide) or weight row (thin)
-        int it = 0;
-        for (int t = blockIdx.x; t < total; t += gridDim.x)
+        Ring<FG_STAGES> sg;
+        Ring<FG_SCALES> sr;
+        int b = 0;                                          // TMEM buffer
+        const uint32_t tempty = in_cta0(&bar_tempty[0]);
+        for (int t = cluster; t < total; t += n_clusters)
         {
-            const Tile ti = tile_at<SWIGLU>(p, s_pref, t);
-            uint64_t acc[2][32];                            // wide: 64 columns of each block; thin: 2 chunks of 16
+            Tile ti = tile_at(p, s_pref, t);
+            uint64_t acc[2][16];                            // 32 columns (wide) or tokens (thin) of each block
             #pragma unroll
             for (int h = 0; h < 2; ++h)
                 #pragma unroll
-                for (int i = 0; i < 32; ++i) acc[h][i] = 0;
+                for (int i = 0; i < 16; ++i) acc[h][i] = 0;
+            const bool work = !ti.thin || g * 32 < ti.rows;
             bool ok = true;
             #pragma unroll 1
-            for (int kb = 0; kb < nkb; ++kb, ++it)
+            for (int kb = 0; kb < nkb; ++kb)
             {
-                const int b = it & 1, q = it % FG_SCALES;
-                if (!mbar_try_wait(&bar_sfull[q], (it / FG_SCALES) & 1u) || !mbar_try_wait(&bar_tfull[b], (it >> 1) & 1u))
-                    ok = mbar_wait(&bar_sfull[q], (it / FG_SCALES) & 1u, abort_flag, p.status, p.wait_ns) &&
-                         mbar_wait(&bar_tfull[b], (it >> 1) & 1u, abort_flag, p.status, p.wait_ns);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                const int q = sr.slot;
+                if (!__all_sync(0xffffffffu, mbar_test_wait2(&bar_sfull[q], sr.parity, &bar_done[sg.slot], sg.parity)))
+                {
+                    ok = warp_wait(&bar_sfull[q], sr.parity, abort_flag, p.status, p.wait_ns) &&
+                         warp_wait(&bar_done[sg.slot], sg.parity, abort_flag, p.status, p.wait_ns);
+                    if (!ok) break;
+                }
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + b * 256;
                 if (!ti.thin)
                 {
+                    const float x = s_sx[q][lane_in];
                     #pragma unroll
                     for (int h = 0; h < 2; ++h)
                     {
-                        const uint32_t f = __float_as_uint(s_scale[q][h][lane_in]);
+                        const uint32_t f = __float_as_uint(x * s_sw[q][h]);
                         const uint64_t ff = pack2(f, f);
                         #pragma unroll
                         for (int c = 0; c < 2; ++c)
                         {
-                            uint64_t d[16];
-                            tmem_load(taddr + h * 128 + g * 64 + c * 32, d);
+                            uint64_t d[8];
+                            tmem_load(taddr + h * 128 + g * 32 + c * 16, d);
                             #pragma unroll
-                            for (int i = 0; i < 16; ++i) fma2(acc[h][c * 16 + i], d[i], ff);
+                            for (int i = 0; i < 8; ++i) fma2(acc[h][c * 8 + i], d[i], ff);
                         }
                     }
                 }
-                else
+                else if (work)
                 {
+                    const float* sc = &s_sx[q][g * 32];
+                    const uint32_t w0 = __float_as_uint(s_sw[q][0]), w1 = __float_as_uint(s_sw[q][1]);
+                    const uint64_t ww[2] = {pack2(w0, w0), pack2(w1, w1)};
                     #pragma unroll
-                    for (int ci = 0; ci < 2; ++ci)
-                        if ((2 * ci + g) * 16 < ti.rows)
+                    for (int c = 0; c < 2; ++c)
+                        if (g * 32 + c * 16 < ti.rows)
                         {
-                            const float* sc = &s_scale[q][0][(2 * ci + g) * 16];
                             #pragma unroll
                             for (int h = 0; h < 2; ++h)
                             {
                                 uint64_t d[8];
-                                tmem_load(taddr + h * 128 + (2 * ci + g) * 16, d);
+                                tmem_load(taddr + h * 128 + g * 32 + c * 16, d);
                                 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
                                 {
-                                    const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + h * NT + 4 * i);
-                                    fma2(acc[h][ci * 8 + 2 * i], d[2 * i], f.x);
-                                    fma2(acc[h][ci * 8 + 2 * i + 1], d[2 * i + 1], f.y);
+                                    const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + c * 16 + 4 * i);
+                                    fma2(acc[h][c * 8 + 2 * i], d[2 * i], mul2(f.x, ww[h]));
+                                    fma2(acc[h][c * 8 + 2 * i + 1], d[2 * i + 1], mul2(f.y, ww[h]));
                                 }
                             }
                         }
@@ -617,72 +690,76 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 __syncwarp();
                 if (lane == 0)
                 {
-                    mbar_arrive(&bar_tempty[b]);
+                    mbar_arrive_cluster(tempty + b * 8);
                     mbar_arrive(&bar_sempty[q]);
                 }
+                b ^= 1;
+                sg.next();
+                sr.next();
             }
             // A warp that gave up says so before the epilogue's barrier, and every warp reads it between this
-            // barrier and the next: one decision for all eight.
+            // barrier and the next: one decision for all of them.
             if (!ok && lane == 0) s_fail = 1;
-            named_bar_sync(3, 256);
+            named_bar_sync(5, FG_EPI_THREADS);
             const bool fail = *(volatile int*) &s_fail != 0;
             if (fail)
             {
-                named_bar_sync(3, 256);
+                named_bar_sync(5, FG_EPI_THREADS);
                 break;
             }
             if (ti.thin)
             {
                 float* st = &s_stage[g][0][0];
                 #pragma unroll
-                for (int ci = 0; ci < 2; ++ci)
-                    #pragma unroll
-                    for (int j0 = 0; j0 < 16; j0 += FG_STEP)
+                for (int j0 = 0; j0 < 32; j0 += FG_STEP)
+                {
+                    const int m0 = g * 32 + j0;
+                    if (m0 < ti.rows)
                     {
-                        const int m0 = (2 * ci + g) * 16 + j0;
-                        if (m0 < ti.rows)
-                        {
+                        #pragma unroll
+                        for (int j = 0; j < FG_STEP; ++j)
                             #pragma unroll
-                            for (int j = 0; j < FG_STEP; ++j)
-                                #pragma unroll
-                                for (int h = 0; h < 2; ++h)
-                                    st[j * 256 + h * 128 + lane_in] = half_of(acc[h][ci * 8 + ((j0 + j) >> 1)], j & 1);
-                            named_bar_sync(1 + g, 128);
-                            write_step<SWIGLU>(p, ti, st, m0, threadIdx.x & 127);
-                            named_bar_sync(1 + g, 128);
-                        }
+                            for (int h = 0; h < 2; ++h)
+                                st[j * 256 + h * 128 + lane_in] = half_of(acc[h][(j0 + j) >> 1], j & 1);
+                        named_bar_sync(1 + g, 128);
+                        write_step<SWIGLU>(p, ti, rank, st, m0, threadIdx.x & 127);
+                        named_bar_sync(1 + g, 128);
                     }
-                named_bar_sync(3, 256);
+                }
+                named_bar_sync(5, FG_EPI_THREADS);
             }
             else if constexpr (!SWIGLU)
             {
+                ti.row0 += 128 * rank;                      // this CTA's tokens
+                ti.rows -= 128 * rank;
                 if (p.out_dtype == 0) store_wide<float>(p, ti, acc, g, lane_in);
                 else if (p.out_dtype == 1) store_wide<__half>(p, ti, acc, g, lane_in);
                 else store_wide<__nv_bfloat16>(p, ti, acc, g, lane_in);
-                named_bar_sync(3, 256);
+                named_bar_sync(5, FG_EPI_THREADS);
             }
             else
             {
-                // this thread's token: 64 of the block's 128 columns; the largest magnitude of the other 64 comes from
-                // the other warpgroup
-                float act[64];
+                // this thread's token: 32 of the block's 128 columns; the largest magnitude of the others comes from
+                // the other warpgroups
+                float act[32];
                 uint32_t mx = 0;
                 #pragma unroll
-                for (int i = 0; i < 64; ++i)
+                for (int i = 0; i < 32; ++i)
                 {
                     act[i] = clamped_swiglu(half_of(acc[0][i >> 1], i & 1), half_of(acc[1][i >> 1], i & 1), p.limit);
                     mx = max(mx, __float_as_uint(act[i]) & 0x7fffffffu);
                 }
+                uint32_t (*s_amax)[NT] = reinterpret_cast<uint32_t (*)[NT]>(&s_stage[0][0][0]);     // thin tiles' memory
                 s_amax[g][lane_in] = mx;
-                named_bar_sync(3, 256);
-                mx = max(mx, s_amax[g ^ 1][lane_in]);
-                if (lane_in < ti.rows)
+                named_bar_sync(5, FG_EPI_THREADS);
+                mx = max(max(s_amax[0][lane_in], s_amax[1][lane_in]), max(s_amax[2][lane_in], s_amax[3][lane_in]));
+                if (128 * rank + lane_in < ti.rows)
                 {
                     const float s = block_scale(__uint_as_float(mx), false), inv = 1.0f / s;
-                    const int64_t r = ti.row0 + lane_in;
-                    uint4* h = reinterpret_cast<uint4*>(p.h + r * p.h_stride + ti.nt * kBlock + g * 64);
+                    const int64_t r = ti.row0 + 128 * rank + lane_in;
+                    uint4* h = reinterpret_cast<uint4*>(p.h + r * p.h_stride + ti.nt * kBlock + g * 32);
                     #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 2; ++c)
                     {
                         uint32_t w[4];
                         #pragma unroll
@@ -701,13 +778,14 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         }
     }
 
-    // ---- teardown
+    // ---- teardown: neither CTA leaves while the other may still use its shared memory or its TMEM
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     if (warp == 1)
     {
         tc_fence_after();
-        tmem_dealloc(tmem_base, TMEM_COLS);
+        tmem_dealloc_pair(tmem_base, TMEM_COLS);
     }
 }
 
@@ -726,6 +804,15 @@ int make_map(CUtensorMap* tmap, const void* base, int rank, const cuuint64_t* di
 }
 
 std::atomic<bool> g_fp8_attr_set[kMaxDevices] = {};
+std::atomic<int> g_fp8_clusters[kMaxDevices] = {};
+
+int max_clusters()
+{
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return device_sm_count() / 2;
+    const int n = g_fp8_clusters[dev].load(std::memory_order_relaxed);
+    return n > 0 ? n : device_sm_count() / 2;
+}
 
 constexpr uint32_t kDynBytes = FG_STAGES * FG_STAGE_BYTES + 1024;
 
@@ -735,12 +822,15 @@ int launch_fp8_gemm(const Fp8GemmProblem& q, cudaStream_t stream)
 {
     Fp8GemmArgs p{};
     p.N = q.N; p.K = q.K; p.n_experts = q.n_experts;
-    p.n_tiles_n = q.swiglu ? q.N / 2 / kBlock : (q.N + 255) / 256;
+    p.n_blocks = (q.N + kBlock - 1) / kBlock;
+    const int units = q.swiglu ? q.N / 2 / kBlock : (p.n_blocks + 1) / 2;   // pairs of blocks that belong together
+    p.n_wide = units;
+    p.n_thin = (units + 1) / 2;
     p.num_kb = (q.K + FG_BK - 1) / FG_BK;
     p.single_count = (int) q.rows;
     p.counts = q.counts; p.row0 = q.row0;
     p.sx = q.sx; p.sx_row = q.sx_row; p.sx_blk = q.sx_blk;
-    p.sw = q.sw; p.sw_expert = q.sw_expert; p.sw_n = q.sw_n; p.sw_k = 1;
+    p.sw = q.sw; p.sw_expert = q.sw_expert; p.sw_n = q.sw_n;
     p.out = q.out; p.out_stride = q.out_stride; p.out_dtype = q.out_dtype; p.accumulate = q.accumulate;
     p.slot = q.slot;
     p.out_vec = reinterpret_cast<uintptr_t>(q.out) % 16 == 0 && q.out_stride * (q.out_dtype == 0 ? 4 : 2) % 16 == 0;
@@ -757,20 +847,30 @@ int launch_fp8_gemm(const Fp8GemmProblem& q, cudaStream_t stream)
     const cuuint64_t xs[1] = {(cuuint64_t) q.x_stride};
     rc = make_map(&tx, q.x, 2, xd, xs, FG_XBOX);
     if (rc) return rc;
-    rc = once_per_device(g_fp8_attr_set, "fp8_gemm", [](int) {
+    rc = once_per_device(g_fp8_attr_set, "fp8_gemm", [](int dev) {
         cudaError_t err = cudaSuccess;
         auto set = [&](const void* fn, uint32_t bytes) {
             if (err == cudaSuccess) err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
         };
         set((const void*) fp8_gemm_kernel<false>, kDynBytes);
         set((const void*) fp8_gemm_kernel<true>, kDynBytes);
-        return err == cudaSuccess ? 0 : set_cuda_error("fp8_gemm: cudaFuncSetAttribute", err);
+        if (err != cudaSuccess) return set_cuda_error("fp8_gemm: cudaFuncSetAttribute", err);
+        // clusters that run at one time (SMs without a partner in their GPC stay out)
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(2 * 1024);
+        cfg.blockDim = dim3(FG_THREADS);
+        cfg.dynamicSmemBytes = kDynBytes;
+        int n = 0;
+        err = cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<true>, &cfg);
+        if (err != cudaSuccess || n < 1) return set_cuda_error("fp8_gemm: cudaOccupancyMaxActiveClusters", err);
+        g_fp8_clusters[dev] = n;
+        return 0;
     });
     if (rc) return rc;
     // tiles are counted on the device; this bound only keeps the grid from being larger than the work
-    const int64_t sms = device_sm_count();
-    const int64_t tiles = (q.rows / NT + (q.rows < q.n_experts ? q.rows : q.n_experts)) * p.n_tiles_n;
-    const unsigned grid = (unsigned) (tiles < sms ? tiles : sms);
+    const int64_t tiles = (q.rows / 256 + (q.rows < q.n_experts ? q.rows : q.n_experts)) * p.n_wide;
+    const int64_t most = max_clusters();
+    const unsigned grid = 2u * (unsigned) (tiles < most ? tiles : most);
     if (q.swiglu) fp8_gemm_kernel<true><<<grid, FG_THREADS, kDynBytes, stream>>>(tw, tx, p);
     else fp8_gemm_kernel<false><<<grid, FG_THREADS, kDynBytes, stream>>>(tw, tx, p);
     return check_launch("fp8_gemm");
