@@ -24,6 +24,11 @@
 //         token.  An expert with few rows costs few columns.  Every value needs its column's scale here, which a warp
 //         reads from shared memory (128 bytes a clock for the SM): 8 clocks per column and K block.
 //
+// A K block is two halves, each with its own pair of TMEM buffers, MMAs and barriers: half j is rows 64 j .. 64 j + 63 of
+// both weight blocks (wide) or tokens 64 j .. (thin), and is worked on by warpgroups 2 j and 2 j + 1.  What bounds
+// the loop is the way round one TMEM buffer (MMA, commit, taking the sums out, arrival, next MMA: about 2000 clocks),
+// and the two halves go round out of step.
+//
 //   warp 0        TMA producer of this CTA's operands: weight blocks [128 x 128 B], token rows in boxes of 32;
 //   warp 1        MMA issuer (in CTA 0, for both), TMEM owner;
 //   warps 2, 3    scales of the coming K blocks into a shared-memory ring (cp.async, up to eight blocks ahead);
@@ -64,7 +69,7 @@ struct Fp8GemmArgs {
     const float* sw; int64_t sw_expert, sw_n;
     // store
     void* out; int64_t out_stride; int out_dtype; int accumulate;
-    int out_vec;                     // rows are 16-byte aligned
+    int out_vec;                     // rows are 32-byte aligned
     const int64_t* slot;             // output row of row r, or null
     // swiglu
     int f; float limit;
@@ -372,6 +377,14 @@ __device__ __forceinline__ void write_step(const Fp8GemmArgs& p, const Tile& ti,
     }
 }
 
+// One whole 32-byte sector.
+__device__ __forceinline__ void store32(void* dst, const uint32_t* w)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :: "l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
 // Wide tiles, store: this thread's token, 32 columns of each of the two weight blocks.
 template <class To>
 __device__ __forceinline__ void store_wide(const Fp8GemmArgs& p, const Tile& ti, const uint64_t (&acc)[2][16], int g, int m)
@@ -389,13 +402,10 @@ __device__ __forceinline__ void store_wide(const Fp8GemmArgs& p, const Tile& ti,
             #pragma unroll
             for (int c = 0; c < 32; c += PER)
             {
-                __align__(16) To w[PER];
+                __align__(32) To w[PER];
                 #pragma unroll
                 for (int i = 0; i < PER; ++i) w[i] = from_float<To>(half_of(acc[h][(c + i) >> 1], i & 1));
-                const uint4* v = reinterpret_cast<const uint4*>(w);
-                uint4* o = reinterpret_cast<uint4*>(row + n0 + c);
-                o[0] = v[0];
-                o[1] = v[1];
+                store32(row + n0 + c, reinterpret_cast<const uint32_t*>(w));
             }
         }
         else
@@ -420,9 +430,10 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     constexpr uint32_t TMEM_COLS = 512;                     // two buffers of 256 columns
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bar_full[FG_STAGES];                // CTA 0: both CTAs' operands of a stage have landed
-    __shared__ uint64_t bar_done[FG_STAGES];                // its MMAs are done: the stage is free, the sums are in TMEM
+    __shared__ uint64_t bar_half[FG_STAGES];                // the MMAs of its first half are done
+    __shared__ uint64_t bar_done[FG_STAGES];                // all its MMAs are done: the stage is free
     __shared__ uint64_t bar_sfull[FG_SCALES], bar_sempty[FG_SCALES];
-    __shared__ uint64_t bar_tempty[2];                      // CTA 0: both CTAs have taken a TMEM buffer's sums out
+    __shared__ uint64_t bar_tempty[4];                      // CTA 0: both CTAs have taken the sums of (half, buffer) out
     __shared__ __align__(16) float s_sx[FG_SCALES][NT];
     __shared__ float s_sw[FG_SCALES][2];
     __shared__ uint32_t s_tmem_base;
@@ -465,6 +476,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             for (int s = 0; s < FG_STAGES; ++s)
             {
                 mbar_init(&bar_full[s], 1);
+                mbar_init(&bar_half[s], 1);
                 mbar_init(&bar_done[s], 1);
             }
             for (int s = 0; s < FG_SCALES; ++s)
@@ -472,7 +484,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 mbar_init(&bar_sfull[s], 64);
                 mbar_init(&bar_sempty[s], FG_EPI_WARPS);
             }
-            for (int b = 0; b < 2; ++b) mbar_init(&bar_tempty[b], 2 * FG_EPI_WARPS);
+            for (int b = 0; b < 4; ++b) mbar_init(&bar_tempty[b], FG_EPI_WARPS);      // half of them, in two CTAs
             s_abort = 0;
             s_fail = 0;
             fence_mbar_init();
@@ -501,14 +513,15 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             for (int t = cluster; ok && t < total; t += n_clusters)
             {
                 const Tile ti = tile_at(p, s_pref, t);
-                // boxes of CTA r and the pair's bytes: wide, one weight block and up to 128 tokens a CTA; thin, two
-                // weight blocks and half of the columns
-                const int half = ti.ncols / 2;
-                const int boxes0 = ti.thin ? (half + FG_XBOX - 1) / FG_XBOX : 4;
+                // rows of this CTA's first and last box, boxes, and the pair's bytes: wide, one weight block and up to
+                // 128 tokens a CTA; thin, two weight blocks and half of the columns of each half
+                const int nc1 = max(ti.ncols - 64, 0), nc0 = ti.ncols - nc1;
+                const int boxes0 = ti.thin ? (nc1 ? 2 : 1) : 4;
                 const int boxes1 = ti.thin ? boxes0 : (ti.rows - 128 + FG_XBOX - 1) / FG_XBOX;
                 const uint32_t bytes = (ti.thin ? 4 : 2) * FG_W_BYTES + (boxes0 + boxes1) * (FG_XBOX * FG_BK);
                 const int boxes = rank ? boxes1 : boxes0;
-                const int row = ti.row0 + rank * (ti.thin ? half : 128);
+                const int row = ti.row0 + rank * (ti.thin ? nc0 / 2 : 128);
+                const int row1 = ti.thin ? ti.row0 + 64 + rank * (nc1 / 2) : row + FG_XBOX;
                 const int w_row0 = weight_block<SWIGLU>(p, ti, rank, ti.thin ? 0 : rank) * kBlock;
                 const int w_row1 = weight_block<SWIGLU>(p, ti, rank, 1) * kBlock;
                 const uint32_t x_off = ti.thin ? 2 * FG_W_BYTES : FG_W_BYTES;
@@ -524,8 +537,9 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                         if (rank == 0) mbar_arrive_expect_tx(&bar_full[st.slot], bytes);
                         tma_pair_3d(w, &tmap_w, kb * FG_BK, w_row0, ti.e, full);
                         if (ti.thin) tma_pair_3d(w + FG_W_BYTES, &tmap_w, kb * FG_BK, w_row1, ti.e, full);
-                        for (int b = 0; b < boxes; ++b)
-                            tma_pair_2d(w + x_off + b * (FG_XBOX * FG_BK), &tmap_x, kb * FG_BK, row + b * FG_XBOX, full);
+                        tma_pair_2d(w + x_off, &tmap_x, kb * FG_BK, row, full);
+                        for (int b = 1; b < boxes; ++b)
+                            tma_pair_2d(w + x_off + b * (FG_XBOX * FG_BK), &tmap_x, kb * FG_BK, row1 + (b - 1) * FG_XBOX, full);
                     }
                     __syncwarp();
                 }
@@ -545,38 +559,47 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 for (int t = cluster; ok && t < total; t += n_clusters)
                 {
                     const Tile ti = tile_at(p, s_pref, t);
-                    const uint32_t idesc = idesc_e4m3_f32(256, ti.thin ? ti.ncols : 256);
+                    const int nc1 = max(ti.ncols - 64, 0), nc0 = ti.ncols - nc1;
                     for (int kb = 0; kb < nkb; ++kb, st.next(), buf.next())
                     {
-                        ok = warp_wait(&bar_tempty[buf.slot], buf.parity ^ 1u, abort_flag, p.status, p.wait_ns) &&
-                             warp_wait(&bar_full[st.slot], st.parity, abort_flag, p.status, p.wait_ns);
+                        ok = warp_wait(&bar_full[st.slot], st.parity, abort_flag, p.status, p.wait_ns);
                         if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t w = smem_u32(smem) + st.slot * FG_STAGE_BYTES;
-                        const uint64_t w_desc = smem_desc_sw128(w);
-                        const uint32_t d = tmem_base + buf.slot * 256;
-                        if (elect_one())
+                        const uint64_t w_desc = smem_desc_sw128(smem_u32(smem) + st.slot * FG_STAGE_BYTES);
+                        #pragma unroll
+                        for (int j = 0; j < 2; ++j)
                         {
-                            if (ti.thin)
+                            ok = warp_wait(&bar_tempty[2 * j + buf.slot], buf.parity ^ 1u, abort_flag, p.status, p.wait_ns);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint32_t d = tmem_base + (2 * j + buf.slot) * 128;
+                            if (elect_one())
                             {
-                                const uint64_t x_desc = w_desc + (2 * FG_W_BYTES >> 4);
-                                #pragma unroll
-                                for (int h = 0; h < 2; ++h)
+                                if (ti.thin)
+                                {
+                                    const int nc = j ? nc1 : nc0;
+                                    const uint32_t idesc = idesc_e4m3_f32(256, nc);
+                                    const uint64_t x_desc = w_desc + (2 * FG_W_BYTES + j * (FG_XBOX * FG_BK) >> 4);
+                                    if (nc)
+                                        #pragma unroll
+                                        for (int h = 0; h < 2; ++h)
+                                            #pragma unroll
+                                            for (int kk = 0; kk < FG_BK / 32; ++kk)
+                                                umma_e4m3_pair(d + h * 64, w_desc + h * (FG_W_BYTES >> 4) + 2 * kk,
+                                                               x_desc + 2 * kk, idesc, kk != 0);
+                                }
+                                else
+                                {
+                                    const uint32_t idesc = idesc_e4m3_f32(256, 128);
+                                    const uint64_t x_desc = w_desc + (FG_W_BYTES >> 4);
                                     #pragma unroll
                                     for (int kk = 0; kk < FG_BK / 32; ++kk)
-                                        umma_e4m3_pair(d + h * 128, w_desc + h * (FG_W_BYTES >> 4) + 2 * kk,
-                                                       x_desc + 2 * kk, idesc, kk != 0);
+                                        umma_e4m3_pair(d, x_desc + 2 * kk, w_desc + j * (64 * FG_BK >> 4) + 2 * kk, idesc, kk != 0);
+                                }
+                                umma_commit_pair(j ? &bar_done[st.slot] : &bar_half[st.slot]);
                             }
-                            else
-                            {
-                                const uint64_t x_desc = w_desc + (FG_W_BYTES >> 4);
-                                #pragma unroll
-                                for (int kk = 0; kk < FG_BK / 32; ++kk)
-                                    umma_e4m3_pair(d, x_desc + 2 * kk, w_desc + 2 * kk, idesc, kk != 0);
-                            }
-                            umma_commit_pair(&bar_done[st.slot]);
+                            __syncwarp();
                         }
-                        __syncwarp();
+                        if (!ok) break;
                     }
                 }
                 // the MMAs of the last stages are done before the CTAs leave: the producer's drain waits for them
@@ -621,7 +644,8 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         Ring<FG_STAGES> sg;
         Ring<FG_SCALES> sr;
         int b = 0;                                          // TMEM buffer
-        const uint32_t tempty = in_cta0(&bar_tempty[0]);
+        const uint32_t tempty = in_cta0(&bar_tempty[2 * (g >> 1)]);
+        uint64_t* bar_sums = g >> 1 ? bar_done : bar_half;
         for (int t = cluster; t < total; t += n_clusters)
         {
             Tile ti = tile_at(p, s_pref, t);
@@ -636,14 +660,15 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             for (int kb = 0; kb < nkb; ++kb)
             {
                 const int q = sr.slot;
-                if (!__all_sync(0xffffffffu, mbar_test_wait2(&bar_sfull[q], sr.parity, &bar_done[sg.slot], sg.parity)))
+                if (!__all_sync(0xffffffffu, mbar_test_wait2(&bar_sfull[q], sr.parity, &bar_sums[sg.slot], sg.parity)))
                 {
                     ok = warp_wait(&bar_sfull[q], sr.parity, abort_flag, p.status, p.wait_ns) &&
-                         warp_wait(&bar_done[sg.slot], sg.parity, abort_flag, p.status, p.wait_ns);
+                         warp_wait(&bar_sums[sg.slot], sg.parity, abort_flag, p.status, p.wait_ns);
                     if (!ok) break;
                 }
                 tc_fence_after();
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + b * 256;
+                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (2 * (g >> 1) + b) * 128 +
+                                       (g & 1) * 32;
                 if (!ti.thin)
                 {
                     const float x = s_sx[q][lane_in];
@@ -656,7 +681,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                         for (int c = 0; c < 2; ++c)
                         {
                             uint64_t d[8];
-                            tmem_load(taddr + h * 128 + g * 32 + c * 16, d);
+                            tmem_load(taddr + h * 64 + c * 16, d);
                             #pragma unroll
                             for (int i = 0; i < 8; ++i) fma2(acc[h][c * 8 + i], d[i], ff);
                         }
@@ -675,7 +700,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                             for (int h = 0; h < 2; ++h)
                             {
                                 uint64_t d[8];
-                                tmem_load(taddr + h * 128 + g * 32 + c * 16, d);
+                                tmem_load(taddr + h * 64 + c * 16, d);
                                 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
                                 {
@@ -833,7 +858,7 @@ int launch_fp8_gemm(const Fp8GemmProblem& q, cudaStream_t stream)
     p.sw = q.sw; p.sw_expert = q.sw_expert; p.sw_n = q.sw_n;
     p.out = q.out; p.out_stride = q.out_stride; p.out_dtype = q.out_dtype; p.accumulate = q.accumulate;
     p.slot = q.slot;
-    p.out_vec = reinterpret_cast<uintptr_t>(q.out) % 16 == 0 && q.out_stride * (q.out_dtype == 0 ? 4 : 2) % 16 == 0;
+    p.out_vec = reinterpret_cast<uintptr_t>(q.out) % 32 == 0 && q.out_stride * (q.out_dtype == 0 ? 4 : 2) % 32 == 0;
     p.f = q.N / 2; p.limit = q.limit;
     p.h = static_cast<uint8_t*>(q.h); p.h_stride = q.h_stride; p.hs = q.hs; p.hs_row = q.hs_row; p.hs_blk = q.hs_blk;
     p.status = q.status;
