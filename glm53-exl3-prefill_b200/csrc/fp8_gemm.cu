@@ -245,6 +245,23 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
     return r;
 }
 
+// Which of three phases are complete (bits 0..2; the same answer for the whole warp), without blocking.
+__device__ __forceinline__ uint32_t mbar_test3(uint64_t* a, uint32_t parity_a, uint64_t* b, uint64_t* c, uint32_t parity_bc)
+{
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred pa, pb, pc;\n\t.reg .b32 x, y;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 pa, [%1], %2;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 pb, [%3], %5;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 pc, [%4], %5;\n\t"
+        "selp.u32 %0, 1, 0, pa;\n\t"
+        "selp.u32 x, 2, 0, pb;\n\t"
+        "selp.u32 y, 4, 0, pc;\n\t"
+        "or.b32 %0, %0, x;\n\tor.b32 %0, %0, y;\n\t}"
+        : "=&r"(r) : "r"(smem_u32(a)), "r"(parity_a), "r"(smem_u32(b)), "r"(smem_u32(c)), "r"(parity_bc) : "memory");
+    return __reduce_and_sync(0xffffffffu, r);
+}
+
 // mbar_wait by a whole warp, with one answer for it.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
                                           uint64_t limit_ns)
@@ -555,6 +572,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             {
                 Ring<FG_STAGES> st;
                 Ring<2> buf;
+                const bool leader = elect_one();
                 bool ok = true;
                 for (int t = cluster; ok && t < total; t += n_clusters)
                 {
@@ -562,18 +580,25 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                     const int nc1 = max(ti.ncols - 64, 0), nc0 = ti.ncols - nc1;
                     for (int kb = 0; kb < nkb; ++kb, st.next(), buf.next())
                     {
-                        ok = warp_wait(&bar_full[st.slot], st.parity, abort_flag, p.status, p.wait_ns);
-                        if (!ok) break;
+                        // one round trip to shared memory for the three barriers of a K block: this warp's own
+                        // instructions are what the loop waits for once the sums keep up
+                        const uint32_t ready = mbar_test3(&bar_full[st.slot], st.parity, &bar_tempty[buf.slot],
+                                                          &bar_tempty[2 + buf.slot], buf.parity ^ 1u);
+                        if (!(ready & 1u))
+                            ok = warp_wait(&bar_full[st.slot], st.parity, abort_flag, p.status, p.wait_ns);
                         const uint64_t w_desc = smem_desc_sw128(smem_u32(smem) + st.slot * FG_STAGE_BYTES);
+                        const uint32_t d0 = tmem_base + buf.slot * 128;
                         #pragma unroll
                         for (int j = 0; j < 2; ++j)
                         {
-                            ok = warp_wait(&bar_tempty[2 * j + buf.slot], buf.parity ^ 1u, abort_flag, p.status, p.wait_ns);
+                            if (!(ready & (2u << j)))
+                                ok = ok && warp_wait(&bar_tempty[2 * j + buf.slot], buf.parity ^ 1u, abort_flag, p.status,
+                                                     p.wait_ns);
                             if (!ok) break;
                             tc_fence_after();
-                            const uint32_t d = tmem_base + (2 * j + buf.slot) * 128;
-                            if (elect_one())
+                            if (leader)
                             {
+                                const uint32_t d = d0 + 256 * j;
                                 if (ti.thin)
                                 {
                                     const int nc = j ? nc1 : nc0;
