@@ -29,32 +29,19 @@ __device__ __forceinline__ float block_scale(float amax, bool pow2)
     return __uint_as_float(e << 23);
 }
 
-// x / scale as a float that rounds to the same e4m3 value as the exact quotient does.  A plain rounded
-// quotient can land on the border between two e4m3 values that the exact one only comes near; where
-// the division is inexact its last bit is made odd, towards the exact quotient (borders have an even one).
-static __device__ __noinline__ float quotient_sticky(float x, float scale)
-{
-    const float q = __fdiv_rn(x, scale);
-    const float r = __fmaf_rn(-q, scale, x);                // exact: the sign of what the rounding lost
-    uint32_t u = __float_as_uint(q);
-    if (r != 0.0f && !(u & 1u) && (u & 0x7fffffffu) < 0x7f800000u && u << 1)
-    {
-        const bool grow = (r > 0.0f) == (x > 0.0f);         // the exact quotient is further from zero
-        u += grow ? 1u : 0xffffffffu;
-    }
-    return __uint_as_float(u);
-}
-
-// The same, cheaply: x * inv is within 2 units in the last place of the quotient, so only products that
-// close to a border between e4m3 values (normal ones: their low 20 bits near 0x80000) need the division.
-// Below 2^-6 the spacing is that of e4m3's subnormals, with borders elsewhere: those are always divided.
+// x / scale as a float that rounds to the same e4m3 value as the exact quotient, with inv = 1 / scale.  The product is
+// corrected once by its remainder, which makes it the rounded quotient; that can still land on the border between
+// two e4m3 values (an even float) when the exact one only comes near, so where a remainder is left the last
+// bit is made odd, towards the exact quotient.  Seven cheap operations: testing for borders first cost more, since with
+// 16-bit inputs every seventh block (a maximum whose bits are a multiple of 7, as 448 is) has exact ties.
 __device__ __forceinline__ float quotient(float x, float scale, float inv)
 {
-    const float v = x * inv;
+    float v = x * inv;
+    v = __fmaf_rn(__fmaf_rn(-v, scale, x), inv, v);
+    const float rest = __fmaf_rn(-v, scale, x);             // exact: the sign of what the rounding lost
     const uint32_t u = __float_as_uint(v);
-    const bool border = ((u + 4u - 0x80000u) & 0xfffffu) <= 8u;
-    const bool small = (u & 0x7fffffffu) < 0x3c800000u && x != 0.0f;
-    return border || small ? quotient_sticky(x, scale) : v;
+    const uint32_t odd = (u + (uint32_t) ((int32_t) (u ^ __float_as_uint(rest)) >> 31)) | 1u;
+    return __uint_as_float(rest != 0.0f ? odd : u);
 }
 
 // Two floats to e4m3 (round to nearest even), a in the low byte.

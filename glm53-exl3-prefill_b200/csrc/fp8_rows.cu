@@ -11,12 +11,11 @@ using namespace fp8;
 //     s[r, b] = max(max_k |x[r, k]|, 2^-64) / 448   (or the least power of two at or above that)
 //     q[r, k] = e4m3(x[r, k] / s[r, k / 128])       b = k / 128
 // bound by bytes: a row is read once (2 or 4 bytes a value) and written once (1 byte).  Eight lanes hold a block,
-// 16 values each, so loads are 32 or 64 bytes and the store 16 bytes a lane, and a block's maximum is three shuffles.
+// 16 values each, so loads are whole 32-byte sectors, the store is 16 bytes a lane, and a block's maximum is three shuffles.
 struct QuantArgs {
     const void* x;
     int64_t x_stride;                // elements
     int K, n_blocks;
-    int pow2;
     uint8_t* q;
     int64_t q_stride;
     float* scale;
@@ -30,50 +29,56 @@ struct QuantArgs {
 
 constexpr int Q_THREADS = 256;
 
-template <class T, bool VEC>
+// 32 bytes from a 32-byte (16-byte) aligned address.
+template <bool ALIGNED32>
+__device__ __forceinline__ void load32(const void* src, uint32_t* w)
+{
+    if constexpr (ALIGNED32)
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(src));
+    else
+    {
+        reinterpret_cast<uint4*>(w)[0] = __ldg(reinterpret_cast<const uint4*>(src));
+        reinterpret_cast<uint4*>(w)[1] = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+    }
+}
+
+// ALIGN: 32 or 16 bytes (rows and K allow vectors), 0: element by element.  Index: type of a (row, block) number.
+template <class T, int ALIGN, bool POW2, class Index>
 __global__ __launch_bounds__(Q_THREADS)
 void quantize_rows_kernel(const QuantArgs p)
 {
     const int lane8 = threadIdx.x & 7;
     const int64_t rows = p.rows_dev ? min(p.rows, (int64_t) *p.rows_dev) : p.rows;
-    const int64_t units = rows * p.n_blocks;                        // (row, block) pairs, blocks fastest
-    const int64_t step = (int64_t) gridDim.x * (Q_THREADS / 8);
+    const Index units = (Index) (rows * p.n_blocks);                // (row, block) pairs, blocks fastest
+    const Index step = (Index) gridDim.x * (Q_THREADS / 8);
     // whole warps take part in the shuffles: the bound is rounded up to the warp's four units
-    const int64_t first = ((int64_t) blockIdx.x * Q_THREADS + threadIdx.x) >> 3;
-    for (int64_t u = first; u - (first & 3) < units; u += step)
+    const Index first = ((Index) blockIdx.x * Q_THREADS + threadIdx.x) >> 3;
+    for (Index u = first; u - (first & 3) < units; u += step)
     {
         const bool live = u < units;
-        const int64_t r = live ? u / p.n_blocks : 0;
-        const int b = live ? (int) (u - r * p.n_blocks) : 0;
-        const int64_t src = p.slot && live ? __ldg(p.slot + r) / p.topk : r;
+        const Index row = live ? u / (Index) p.n_blocks : 0;
+        const int b = live ? (int) (u - row * (Index) p.n_blocks) : 0;
+        const int64_t r = (int64_t) row;
+        const int64_t src = p.slot && live ? (int64_t) ((uint32_t) __ldg(p.slot + r) / (uint32_t) p.topk) : r;
         const int k0 = b * kBlock + lane8 * 16;
         const T* x = reinterpret_cast<const T*>(p.x) + src * p.x_stride + k0;
         float v[16];
-        #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-        if (live)
+        if (live && ALIGN && k0 < p.K)                              // K % 16 == 0
         {
-            if (VEC)                                                // K % 16 == 0, rows 16-byte aligned
-            {
-                if (k0 < p.K)
-                {
-                    constexpr int PER = 16 / sizeof(T);
-                    #pragma unroll
-                    for (int j = 0; j < 16 / PER; ++j)
-                    {
-                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(x) + j);
-                        const T* h = reinterpret_cast<const T*>(&w);
-                        #pragma unroll
-                        for (int i = 0; i < PER; ++i) v[j * PER + i] = to_float(h[i]);
-                    }
-                }
-            }
-            else
-            {
-                #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (k0 + i < p.K) v[i] = to_float(x[i]);
-            }
+            __align__(16) uint32_t w[4 * sizeof(T)];
+            #pragma unroll
+            for (int j = 0; j < (int) sizeof(T) / 2; ++j)
+                load32<ALIGN == 32>(reinterpret_cast<const uint8_t*>(x) + 32 * j, w + 8 * j);
+            const T* h = reinterpret_cast<const T*>(w);
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = to_float(h[i]);
+        }
+        else
+        {
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = !ALIGN && live && k0 + i < p.K ? to_float(x[i]) : 0.0f;
         }
         uint32_t m = 0;                                             // magnitudes as integers: NaN is the largest
         #pragma unroll
@@ -81,19 +86,15 @@ void quantize_rows_kernel(const QuantArgs p)
         #pragma unroll
         for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (!live) continue;
-        const float s = block_scale(__uint_as_float(m), p.pow2 != 0);
+        const float s = block_scale(__uint_as_float(m), POW2);
         const float inv = 1.0f / s;
         uint32_t w[4];
         #pragma unroll
-        for (int j = 0; j < 4; ++j)
-        {
-            float f[4];
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = quotient(v[4 * j + i], s, inv);
-            w[j] = to_e4m3x2(f[0], f[1]) | to_e4m3x2(f[2], f[3]) << 16;
-        }
+        for (int i = 0; i < 16; ++i) v[i] = POW2 ? v[i] * inv : quotient(v[i], s, inv);    // powers of two: exact
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = to_e4m3x2(v[4 * j], v[4 * j + 1]) | to_e4m3x2(v[4 * j + 2], v[4 * j + 3]) << 16;
         uint8_t* q = p.q + r * p.q_stride + k0;
-        if (VEC)
+        if (ALIGN)
         {
             if (k0 < p.K) *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -160,11 +161,20 @@ void combine_routes_kernel(const CombineArgs p)
     for (int i = 0; i < 4; ++i) out[i] = from_float<To>(a[i]);
 }
 
-template <class T>
-void launch_quant(const QuantArgs& p, bool vec, unsigned grid, cudaStream_t stream)
+template <class T, int ALIGN>
+void launch_quant(const QuantArgs& p, bool pow2, unsigned grid, cudaStream_t stream)
 {
-    if (vec) quantize_rows_kernel<T, true><<<grid, Q_THREADS, 0, stream>>>(p);
-    else quantize_rows_kernel<T, false><<<grid, Q_THREADS, 0, stream>>>(p);
+    const bool small = p.rows * p.n_blocks < (1LL << 31);           // (row, block) numbers fit 32 bits: cheap divisions
+    if (pow2)
+    {
+        if (small) quantize_rows_kernel<T, ALIGN, true, uint32_t><<<grid, Q_THREADS, 0, stream>>>(p);
+        else quantize_rows_kernel<T, ALIGN, true, uint64_t><<<grid, Q_THREADS, 0, stream>>>(p);
+    }
+    else
+    {
+        if (small) quantize_rows_kernel<T, ALIGN, false, uint32_t><<<grid, Q_THREADS, 0, stream>>>(p);
+        else quantize_rows_kernel<T, ALIGN, false, uint64_t><<<grid, Q_THREADS, 0, stream>>>(p);
+    }
 }
 
 }  // namespace
@@ -174,18 +184,25 @@ int launch_fp8_quantize(const void* x, int dtype, int64_t rows, int K, int64_t x
                         const int32_t* rows_dev, cudaStream_t stream)
 {
     QuantArgs p{};
-    p.x = x; p.x_stride = x_stride; p.K = K; p.n_blocks = (K + kBlock - 1) / kBlock; p.pow2 = pow2;
+    p.x = x; p.x_stride = x_stride; p.K = K; p.n_blocks = (K + kBlock - 1) / kBlock;
     p.q = static_cast<uint8_t*>(q); p.q_stride = q_stride; p.scale = scale; p.s_row = s_row; p.s_blk = s_blk;
     p.rows = rows; p.slot = slot; p.topk = topk; p.rows_dev = rows_dev;
     const int64_t size = dtype == 0 ? 4 : 2;
-    const bool vec = K % 16 == 0 && (x_stride * size) % 16 == 0 && q_stride % 16 == 0 &&
-                     reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(x) | (uintptr_t) (x_stride * size);
+    int align = K % 16 == 0 && q_stride % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 ? 32 : 0;
+    if (at % 32 != 0) align = align && at % 16 == 0 ? 16 : 0;
     const int64_t ctas = (rows * p.n_blocks + Q_THREADS / 8 - 1) / (Q_THREADS / 8);
     const int64_t most = (int64_t) device_sm_count() * 64;
     const unsigned grid = (unsigned) (ctas < most ? ctas : most);
-    if (dtype == 0) launch_quant<float>(p, vec, grid, stream);
-    else if (dtype == 1) launch_quant<__half>(p, vec, grid, stream);
-    else launch_quant<__nv_bfloat16>(p, vec, grid, stream);
+    auto go = [&](auto v) {
+        using T = decltype(v);
+        if (align == 32) launch_quant<T, 32>(p, pow2 != 0, grid, stream);
+        else if (align == 16) launch_quant<T, 16>(p, pow2 != 0, grid, stream);
+        else launch_quant<T, 0>(p, pow2 != 0, grid, stream);
+    };
+    if (dtype == 0) go(float{});
+    else if (dtype == 1) go(__half{});
+    else go(__nv_bfloat16{});
     return check_launch("fp8_quantize_rows");
 }
 
