@@ -70,6 +70,10 @@ ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_
     return b;
 }
 
+// Routes whose products each read their expert's weights for themselves (fp8_small.cu), activations [R, f] in the workspace.
+constexpr int64_t kFewRoutes = 32;
+bool few_routes(int64_t R) { return R <= kFewRoutes; }
+
 int check_rows(const char* what, int64_t dtype, int64_t rows, int64_t K, int64_t stride)
 {
     if (!is_dtype(dtype)) return set_error("%s: unknown dtype", what);
@@ -189,6 +193,9 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     if (w_scale_stride < blocks128(K)) return set_error("fp8_linear: weight scales [ceil(N / 128), ceil(K / 128)]");
     if (!aligned16(workspace) || workspace_bytes < exl3_fp8_linear_workspace(T, K))
         return set_error("fp8_linear: workspace must hold exl3_fp8_linear_workspace() bytes");
+    if (T == 1)
+        return launch_fp8_linear_token(x, (int) dtype, (int) K, w, w_stride, w_scale, w_scale_stride, (int) N, out,
+                                       (int) out_dtype, accumulate ? 1 : 0, as_stream(stream));
     Carver c{static_cast<uint8_t*>(workspace)};
     const Rows8 r = take_rows(c, T, K);
     rc = launch_fp8_quantize(x, (int) dtype, T, (int) K, x_stride, 0, r.q, K, r.s, 1, T, nullptr, 1, nullptr,
@@ -201,7 +208,7 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     p.sw = w_scale; p.sw_n = w_scale_stride; p.sw_expert = 0;
     p.out = out; p.out_stride = out_stride; p.out_dtype = (int) out_dtype; p.accumulate = accumulate ? 1 : 0;
     p.status = status;
-    return launch_fp8_gemm(p, as_stream(stream));
+    return T <= kFp8FewTokens ? launch_fp8_linear_tokens(p, as_stream(stream)) : launch_fp8_gemm(p, as_stream(stream));
 }
 
 int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f)
@@ -240,6 +247,7 @@ int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_s
 int64_t exl3_fp8_experts_workspace(int64_t T, int64_t topk, int64_t E, int64_t d, int64_t f)
 {
     if (check_experts_shape("fp8_experts", T, topk, E, d, f)) return -1;
+    if (few_routes(T * topk)) return up256(T * topk * f * (int64_t) sizeof(float));
     Carver c{nullptr};
     take_experts(c, T, topk, E, d, f);
     return c.used;
@@ -262,10 +270,15 @@ int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t
     if (!aligned16(w13) || !aligned16(w2)) return set_error("fp8_experts: weights must be 16-byte aligned");
     if (!aligned16(workspace) || workspace_bytes < exl3_fp8_experts_workspace(T, topk, E, d, f))
         return set_error("fp8_experts: workspace must hold exl3_fp8_experts_workspace() bytes");
+    cudaStream_t st = as_stream(stream);
+    const int64_t R = T * topk;
+    if (few_routes(R))
+        return launch_fp8_experts_small(x, (int) dtype, (int) T, (int) d, x_stride, ids, ids_is_int64 ? 1 : 0, weights,
+                                        (int) weight_dtype, (int) topk, (int) E, w13, w13_scale, w2, w2_scale, (int) f,
+                                        (float) limit, static_cast<float*>(workspace), out, (int) out_dtype, out_stride,
+                                        accumulate ? 1 : 0, st);
     Carver c{static_cast<uint8_t*>(workspace)};
     const ExpertBuffers b = take_experts(c, T, topk, E, d, f);
-    const int64_t R = T * topk;
-    cudaStream_t st = as_stream(stream);
     // sorted by routing slot t * topk + j, so that each row knows both its token and its place in y
     rc = launch_route_sort(ids, ids_is_int64 ? 1 : 0, weights, (int) weight_dtype, R, 1, (int) E, 0, b.slot,
                            b.weight_sorted, b.expert_of_row, b.counts, b.row0, nullptr, nullptr, b.meta, nullptr,
