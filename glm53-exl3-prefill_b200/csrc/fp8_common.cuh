@@ -21,15 +21,29 @@ constexpr float kAmaxMin = 5.421010862427522e-20f;      // 2^-64: the block maxi
 __device__ __forceinline__ float block_scale(float amax, bool pow2)
 {
     amax = amax < kAmaxMin ? kAmaxMin : amax;
-    if (!pow2) return __fdiv_rn(amax, kE4m3Max);
     const uint32_t u = __float_as_uint(amax);
     if (u >= 0x7f800000u) return amax;
+    if (!pow2)
+    {
+        // amax / 448 rounded, as a product with the rounded 1 / 448 corrected by its remainder
+        constexpr float r = 1.0f / kE4m3Max;
+        const float s = amax * r;
+        return __fmaf_rn(__fmaf_rn(-s, kE4m3Max, amax), r, s);
+    }
     // 448 = 1.75 * 2^8; amax = f * 2^p with 1 <= f < 2: 2^(p-8) while f <= 1.75, else 2^(p-7)
     const uint32_t e = (u >> 23) - 8u + ((u & 0x7fffffu) > 0x600000u ? 1u : 0u);
     return __uint_as_float(e << 23);
 }
 
-// x / scale as a float that rounds to the same e4m3 value as the exact quotient, with inv = 1 / scale.  The product is
+// 1 / s to a unit or so in the last place (s is normal, inf or NaN): quotient() corrects what it is used for.
+__device__ __forceinline__ float reciprocal(float s)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    return r;
+}
+
+// x / scale as a float that rounds to the same e4m3 value as the exact quotient, with inv near 1 / scale.  The product is
 // corrected once by its remainder, which makes it the rounded quotient; that can still land on the border between
 // two e4m3 values (an even float) when the exact one only comes near, so where a remainder is left the last
 // bit is made odd, towards the exact quotient.  Seven cheap operations: testing for borders first cost more, since with

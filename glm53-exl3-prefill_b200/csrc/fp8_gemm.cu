@@ -383,7 +383,7 @@ __device__ __forceinline__ void write_step(const Fp8GemmArgs& p, const Tile& ti,
         mx = __reduce_max_sync(0xffffffffu, mx);
         const int fb = 2 * ti.nt + r0;
         if (m >= ti.rows || fb * kBlock >= p.f) return;
-        const float s = block_scale(__uint_as_float(mx), false), inv = 1.0f / s;
+        const float s = block_scale(__uint_as_float(mx), false), inv = reciprocal(s);
         const int64_t r = ti.row0 + m;
         float q[4];
         #pragma unroll
@@ -805,7 +805,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 mx = max(max(s_amax[0][lane_in], s_amax[1][lane_in]), max(s_amax[2][lane_in], s_amax[3][lane_in]));
                 if (128 * rank + lane_in < ti.rows)
                 {
-                    const float s = block_scale(__uint_as_float(mx), false), inv = 1.0f / s;
+                    const float s = block_scale(__uint_as_float(mx), false), inv = reciprocal(s);
                     const int64_t r = ti.row0 + 128 * rank + lane_in;
                     uint4* h = reinterpret_cast<uint4*>(p.h + r * p.h_stride + ti.nt * kBlock + g * 32);
                     #pragma unroll

@@ -49,6 +49,7 @@ template <class T, int ALIGN, bool POW2, class Index>
 __global__ __launch_bounds__(Q_THREADS)
 void quantize_rows_kernel(const QuantArgs p)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // a product that follows may fetch its weights
     const int lane8 = threadIdx.x & 7;
     const int64_t rows = p.rows_dev ? min(p.rows, (int64_t) *p.rows_dev) : p.rows;
     const Index units = (Index) (rows * p.n_blocks);                // (row, block) pairs, blocks fastest
@@ -87,7 +88,7 @@ void quantize_rows_kernel(const QuantArgs p)
         for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (!live) continue;
         const float s = block_scale(__uint_as_float(m), POW2);
-        const float inv = 1.0f / s;
+        const float inv = POW2 ? 1.0f / s : reciprocal(s);
         uint32_t w[4];
         #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = POW2 ? v[i] * inv : quotient(v[i], s, inv);    // powers of two: exact

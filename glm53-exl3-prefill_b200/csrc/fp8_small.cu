@@ -31,26 +31,36 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The lane's 32 bytes of a row's K block `kb`: bytes 32 t .. 32 t + 31, zeros past K (a multiple of 16).
-template <bool ALIGNED32>
+// The lane's 32 bytes of a row's K block `kb`: bytes 32 t .. 32 t + 31, zeros past K (a multiple of 16).  CONST: memory that
+// nothing writes while the kernel runs (weights), for the read-only path.
+template <bool ALIGNED32, bool CONST>
 __device__ __forceinline__ void load_frag(const uint8_t* row, int kb, int t, int K, uint32_t (&w)[8])
 {
     const int k = kb * kBlock + 32 * t;
     if (ALIGNED32 && k + 32 <= K)
     {
-        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                     : "l"(row + k));
+        if constexpr (CONST)
+            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(row + k));
+        else
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(row + k) : "memory");
         return;
     }
     #pragma unroll
     for (int i = 0; i < 2; ++i)
     {
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (k + 16 * i < K) v = __ldg(reinterpret_cast<const uint4*>(row + k) + i);
+        if (k + 16 * i < K) v = reinterpret_cast<const uint4*>(row + k)[i];
         w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
     }
 }
+
+// Programmatic dependent launch: let the next launch of the stream start; wait for the previous one's results.
+__device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Four consecutive values of a block (columns 4 lane .. 4 lane + 3 of block kb), zeros past K.  `vec`: 4-value loads.
 template <class T>
@@ -84,7 +94,7 @@ __device__ __forceinline__ float quantize_block(const float (&v)[4], int lane, u
     uint32_t m = 0;
     #pragma unroll
     for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    const float s = block_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, m)), false), inv = 1.0f / s;
+    const float s = block_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, m)), false), inv = reciprocal(s);
     float q[4];
     #pragma unroll
     for (int i = 0; i < 4; ++i) q[i] = quotient(v[i], s, inv);
@@ -102,42 +112,54 @@ __device__ __forceinline__ float quantize_block(const float (&v)[4], int lane, u
 __device__ __forceinline__ void block_sums(const uint32_t (&lo)[8], const uint32_t (&hi)[8], const uint32_t (&b)[8],
                                            float (&c)[4])
 {
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};                  // two chains of two: half the latency
     c[0] = c[1] = c[2] = c[3] = 0.0f;
     #pragma unroll
-    for (int i = 0; i < 4; ++i) mma_e4m3(c, lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], b[2 * i], b[2 * i + 1]);
+    for (int i = 0; i < 4; i += 2)
+    {
+        mma_e4m3(c, lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], b[2 * i], b[2 * i + 1]);
+        mma_e4m3(o, lo[2 * i + 2], hi[2 * i + 2], lo[2 * i + 3], hi[2 * i + 3], b[2 * i + 2], b[2 * i + 3]);
+    }
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] += o[i];
 }
 
 // One token by NR tiles of 16 weight rows, K blocks kb0, kb0 + step, ... < kb1: acc[r][0], acc[r][1] = rows g and g + 8 of
-// tile r, in the lanes with t = 0.  row[r][i]: this lane's weight rows; sw[r]: the tile's scales by K block.
-template <int NR, int UNROLL, bool ALIGNED32, class T>
+// tile r, in the lanes with t = 0.  row[r][i]: this lane's weight rows; sw[r]: the tile's scales by K block.  DEPTH
+// blocks of weights are in flight per warp; the first of them before the launch this one depends on has ended
+// (x is only read after it).
+template <int NR, int DEPTH, bool ALIGNED32, class T>
 __device__ __forceinline__ void stream_token(const uint8_t* const (&row)[NR][2], const float* const (&sw)[NR], const T* x,
                                              bool vec, int K, int kb0, int kb1, int step, int lane, float (&acc)[NR][2])
 {
     const int t = lane & 3;
+    uint32_t a[DEPTH][NR][2][8];
+    float f[DEPTH][NR], v[DEPTH][4];
+    auto load_w = [&](int u, int kb) {
+        if (kb >= kb1) return;
+        #pragma unroll
+        for (int r = 0; r < NR; ++r)
+        {
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) load_frag<ALIGNED32, true>(row[r][i], kb, t, K, a[u][r][i]);
+            f[u][r] = __ldg(sw[r] + kb);
+        }
+    };
     #pragma unroll
     for (int r = 0; r < NR; ++r) acc[r][0] = acc[r][1] = 0.0f;
-    for (int kb = kb0; kb < kb1; kb += UNROLL * step)
+    #pragma unroll
+    for (int u = 0; u < DEPTH; ++u) load_w(u, kb0 + u * step);
+    wait_for_previous_launch();
+    #pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+        if (kb0 + u * step < kb1) load_values(x, kb0 + u * step, lane, K, vec, v[u]);
+    for (int kb = kb0; kb < kb1; kb += DEPTH * step)
     {
-        uint32_t a[UNROLL][NR][2][8];
-        float f[UNROLL][NR], v[UNROLL][4];
         #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+        for (int u = 0; u < DEPTH; ++u)
         {
-            const int k = kb + u * step;
+            const int k = kb + u * step, next = k + DEPTH * step;
             if (k >= kb1) break;
-            #pragma unroll
-            for (int r = 0; r < NR; ++r)
-            {
-                #pragma unroll
-                for (int i = 0; i < 2; ++i) load_frag<ALIGNED32>(row[r][i], k, t, K, a[u][r][i]);
-                f[u][r] = __ldg(sw[r] + k);
-            }
-            load_values(x, k, lane, K, vec, v[u]);
-        }
-        #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-        {
-            if (kb + u * step >= kb1) break;
             uint32_t b[8];
             const float s = quantize_block(v[u], lane, b);
             #pragma unroll
@@ -148,6 +170,8 @@ __device__ __forceinline__ void stream_token(const uint8_t* const (&row)[NR][2],
                 acc[r][0] = fmaf(c[0], s * f[u][r], acc[r][0]);
                 acc[r][1] = fmaf(c[2], s * f[u][r], acc[r][1]);
             }
+            load_w(u, next);
+            if (next < kb1) load_values(x, next, lane, K, vec, v[u]);
         }
     }
 }
@@ -217,7 +241,7 @@ template <int NG, bool ALIGNED32>
 __global__ __launch_bounds__(S_THREADS, 2)
 void linear_tokens_kernel(const SmallLinearArgs p)
 {
-    constexpr int UNROLL = NG == 1 ? 4 : 2;
+    constexpr int DEPTH = NG == 1 ? 4 : 2;
     __shared__ float s_sum[S_WARPS][16][NG * 8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * 16, g = lane >> 2, t = lane & 3;
@@ -228,43 +252,40 @@ void linear_tokens_kernel(const SmallLinearArgs p)
     float acc[NG][4];
     #pragma unroll
     for (int j = 0; j < NG; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-    for (int kb = warp; kb < nkb; kb += UNROLL * S_WARPS)
+    uint32_t a[DEPTH][2][8];
+    float f[DEPTH];
+    auto load_w = [&](int u, int kb) {
+        if (kb >= nkb) return;
+        load_frag<ALIGNED32, true>(row0, kb, t, p.K, a[u][0]);
+        load_frag<ALIGNED32, true>(row1, kb, t, p.K, a[u][1]);
+        f[u] = __ldg(sw + kb);
+    };
+    #pragma unroll
+    for (int u = 0; u < DEPTH; ++u) load_w(u, warp + u * S_WARPS);
+    wait_for_previous_launch();
+    for (int kb = warp; kb < nkb; kb += DEPTH * S_WARPS)
     {
-        uint32_t a[UNROLL][2][8], b[UNROLL][NG][8];
-        float f[UNROLL], s[UNROLL][NG][2];
         #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+        for (int u = 0; u < DEPTH; ++u)
         {
             const int k = kb + u * S_WARPS;
             if (k >= nkb) break;
-            load_frag<ALIGNED32>(row0, k, t, p.K, a[u][0]);
-            load_frag<ALIGNED32>(row1, k, t, p.K, a[u][1]);
-            f[u] = __ldg(sw + k);
             #pragma unroll
             for (int j = 0; j < NG; ++j)
             {
                 // a column past the last token repeats it; its sums are not stored
-                load_frag<ALIGNED32>(p.q + (int64_t) min(8 * j + g, p.T - 1) * p.q_stride, k, t, p.K, b[u][j]);
-                #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    s[u][j][i] = __ldg(p.sx + min(8 * j + 2 * t + i, p.T - 1) * p.sx_row + k * p.sx_blk);
-            }
-        }
-        #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-        {
-            if (kb + u * S_WARPS >= nkb) break;
-            #pragma unroll
-            for (int j = 0; j < NG; ++j)
-            {
+                uint32_t b[8];
+                load_frag<ALIGNED32, false>(p.q + (int64_t) min(8 * j + g, p.T - 1) * p.q_stride, k, t, p.K, b);
+                const float f0 = p.sx[min(8 * j + 2 * t, p.T - 1) * p.sx_row + k * p.sx_blk] * f[u];
+                const float f1 = p.sx[min(8 * j + 2 * t + 1, p.T - 1) * p.sx_row + k * p.sx_blk] * f[u];
                 float c[4];
-                block_sums(a[u][0], a[u][1], b[u][j], c);
-                const float f0 = s[u][j][0] * f[u], f1 = s[u][j][1] * f[u];
+                block_sums(a[u][0], a[u][1], b, c);
                 acc[j][0] = fmaf(c[0], f0, acc[j][0]);
                 acc[j][1] = fmaf(c[1], f1, acc[j][1]);
                 acc[j][2] = fmaf(c[2], f0, acc[j][2]);
                 acc[j][3] = fmaf(c[3], f1, acc[j][3]);
             }
+            load_w(u, k + DEPTH * S_WARPS);
         }
     }
     #pragma unroll
@@ -323,6 +344,7 @@ void gate_up_token_kernel(const SmallExpertArgs p)
     __shared__ float s_sum[S_WARPS][32];
     const int64_t slot = blockIdx.y;
     const int64_t e = route_expert(p, slot);
+    let_next_launch_start();
     if (e < 0 || e >= p.E) return;                                  // no expert: the combine leaves the route out
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int n0 = blockIdx.x * 16, nkb = p.d / kBlock;
@@ -332,8 +354,8 @@ void gate_up_token_kernel(const SmallExpertArgs p)
                                       {w + (int64_t) (p.f + n0 + g) * p.d, w + (int64_t) (p.f + n0 + g + 8) * p.d}};
     const float* const sw[2] = {s + (n0 / kBlock) * nkb, s + ((p.f + n0) / kBlock) * nkb};
     float acc[2][2];
-    stream_token<2, 2, true>(row, sw, reinterpret_cast<const T*>(p.x) + slot / p.topk * p.x_stride, p.vec != 0, p.d, warp,
-                             nkb, S_WARPS, lane, acc);
+    stream_token<2, 1, true>(row, sw, reinterpret_cast<const T*>(p.x) + slot / p.topk * p.x_stride, p.vec != 0, p.d,
+                             warp * nkb / S_WARPS, (warp + 1) * nkb / S_WARPS, 1, lane, acc);
     if ((lane & 3) == 0)
         #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -360,7 +382,7 @@ void gate_up_token_kernel(const SmallExpertArgs p)
 __global__ __launch_bounds__(S_THREADS, 2)
 void down_token_kernel(const SmallExpertArgs p)
 {
-    __shared__ float s_sum[32 * S_WARPS][16];                       // [unit][row]: at most topk * parts units
+    __shared__ float s_sum[32][16];                                 // [unit][row]: topk * parts units, at most 32
     const int64_t t = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int n0 = blockIdx.x * 16, nkb = p.f / kBlock;
@@ -374,13 +396,15 @@ void down_token_kernel(const SmallExpertArgs p)
         const uint8_t* const row[1][2] = {{w + (int64_t) (n0 + g) * p.f, w + (int64_t) (n0 + g + 8) * p.f}};
         const float* const sw[1] = {p.s2 + (e * (p.d / kBlock) + n0 / kBlock) * nkb};
         float acc[1][2];
-        stream_token<1, 4, true>(row, sw, p.act + slot * p.f, true, p.f, u % parts, nkb, parts, lane, acc);
+        stream_token<1, 4, true>(row, sw, p.act + slot * p.f, true, p.f, u % parts * nkb / parts,
+                                   (u % parts + 1) * nkb / parts, 1, lane, acc);
         if ((lane & 3) == 0)
         {
             s_sum[u][g] = acc[0][0];
             s_sum[u][g + 8] = acc[0][1];
         }
     }
+    wait_for_previous_launch();                                     // (a warp without a unit has not)
     __syncthreads();
     if (threadIdx.x < 16)
     {
@@ -396,6 +420,24 @@ void down_token_kernel(const SmallExpertArgs p)
         }
         put(p.out, p.out_dtype, t * p.out_stride + n0 + threadIdx.x, sum, p.accumulate != 0);
     }
+}
+
+// A launch that may start before the one in front of it on the stream has ended (its kernel waits for that itself).
+template <class Args>
+int launch_dependent(void (*kernel)(Args), dim3 grid, cudaStream_t stream, const Args& args, const char* what)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(S_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, args);
+    if (err != cudaSuccess) return set_cuda_error(what, err);
+    return check_launch(what);
 }
 
 }  // namespace
@@ -431,17 +473,12 @@ int launch_fp8_linear_tokens(const Fp8GemmProblem& q, cudaStream_t stream)
     const bool a32 = reinterpret_cast<uintptr_t>(q.w) % 32 == 0 && q.w_stride % 32 == 0 &&
                      reinterpret_cast<uintptr_t>(q.x) % 32 == 0 && q.x_stride % 32 == 0;
     const unsigned grid = (unsigned) ((q.N + 15) / 16);
+    const char* what = "fp8_linear (few tokens)";
     if (q.rows <= 8)
-    {
-        if (a32) linear_tokens_kernel<1, true><<<grid, S_THREADS, 0, stream>>>(p);
-        else linear_tokens_kernel<1, false><<<grid, S_THREADS, 0, stream>>>(p);
-    }
-    else
-    {
-        if (a32) linear_tokens_kernel<2, true><<<grid, S_THREADS, 0, stream>>>(p);
-        else linear_tokens_kernel<2, false><<<grid, S_THREADS, 0, stream>>>(p);
-    }
-    return check_launch("fp8_linear (few tokens)");
+        return a32 ? launch_dependent(linear_tokens_kernel<1, true>, dim3(grid), stream, p, what)
+                   : launch_dependent(linear_tokens_kernel<1, false>, dim3(grid), stream, p, what);
+    return a32 ? launch_dependent(linear_tokens_kernel<2, true>, dim3(grid), stream, p, what)
+               : launch_dependent(linear_tokens_kernel<2, false>, dim3(grid), stream, p, what);
 }
 
 int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_stride, const void* ids, int ids_i64,
@@ -463,8 +500,8 @@ int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_s
     else gate_up_token_kernel<__nv_bfloat16><<<grid, S_THREADS, 0, stream>>>(p);
     int rc = check_launch("fp8_experts (gate and up, few routes)");
     if (rc) return rc;
-    down_token_kernel<<<dim3((unsigned) (d / 16), (unsigned) T), S_THREADS, 0, stream>>>(p);
-    return check_launch("fp8_experts (down, few routes)");
+    return launch_dependent(down_token_kernel, dim3((unsigned) (d / 16), (unsigned) T), stream, p,
+                            "fp8_experts (down, few routes)");
 }
 
 }  // namespace exl3b
