@@ -20,8 +20,10 @@ namespace {
 
 using namespace fp8;
 
-constexpr int S_WARPS = 8;
+constexpr int S_WARPS = 8;                      // gate and up
 constexpr int S_THREADS = S_WARPS * 32;
+constexpr int T_WARPS = 16;                     // linear, down: a warp has half as many rows
+constexpr int T_THREADS = T_WARPS * 32;
 
 __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1)
@@ -208,10 +210,10 @@ __device__ __forceinline__ void put(void* out, int dtype, int64_t at, float v, b
 }
 
 template <bool ALIGNED32, class T>
-__global__ __launch_bounds__(S_THREADS, 2)
+__global__ __launch_bounds__(T_THREADS, 2)
 void linear_token_kernel(const SmallLinearArgs p)
 {
-    __shared__ float s_sum[S_WARPS][16];
+    __shared__ float s_sum[T_WARPS][16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * 16, g = lane >> 2;
     const int nkb = (p.K + kBlock - 1) / kBlock;
@@ -219,7 +221,8 @@ void linear_token_kernel(const SmallLinearArgs p)
                                        p.w + (int64_t) min(n0 + g + 8, p.N - 1) * p.w_stride}};
     const float* const sw[1] = {p.sw + (n0 / kBlock) * p.sw_n};
     float acc[1][2];
-    stream_token<1, 4, ALIGNED32>(row, sw, reinterpret_cast<const T*>(p.x), p.vec != 0, p.K, warp, nkb, S_WARPS, lane, acc);
+    stream_token<1, 1, ALIGNED32>(row, sw, reinterpret_cast<const T*>(p.x), p.vec != 0, p.K, warp * nkb / T_WARPS,
+                                   (warp + 1) * nkb / T_WARPS, 1, lane, acc);
     if ((lane & 3) == 0)
     {
         s_sum[warp][g] = acc[0][0];
@@ -231,18 +234,18 @@ void linear_token_kernel(const SmallLinearArgs p)
     {
         float v = 0.0f;
         #pragma unroll
-        for (int w = 0; w < S_WARPS; ++w) v += s_sum[w][threadIdx.x];
+        for (int w = 0; w < T_WARPS; ++w) v += s_sum[w][threadIdx.x];
         put(p.out, p.out_dtype, n, v, p.accumulate != 0);
     }
 }
 
 // 2..16 tokens: NG groups of 8 columns.
 template <int NG, bool ALIGNED32>
-__global__ __launch_bounds__(S_THREADS, 2)
+__global__ __launch_bounds__(T_THREADS, 2)
 void linear_tokens_kernel(const SmallLinearArgs p)
 {
-    constexpr int DEPTH = NG == 1 ? 4 : 2;
-    __shared__ float s_sum[S_WARPS][16][NG * 8];
+    constexpr int DEPTH = 1;
+    __shared__ float s_sum[T_WARPS][16][NG * 8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * 16, g = lane >> 2, t = lane & 3;
     const int nkb = (p.K + kBlock - 1) / kBlock;
@@ -252,24 +255,25 @@ void linear_tokens_kernel(const SmallLinearArgs p)
     float acc[NG][4];
     #pragma unroll
     for (int j = 0; j < NG; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+    const int kb0 = warp * nkb / T_WARPS, kb1 = (warp + 1) * nkb / T_WARPS;
     uint32_t a[DEPTH][2][8];
     float f[DEPTH];
     auto load_w = [&](int u, int kb) {
-        if (kb >= nkb) return;
+        if (kb >= kb1) return;
         load_frag<ALIGNED32, true>(row0, kb, t, p.K, a[u][0]);
         load_frag<ALIGNED32, true>(row1, kb, t, p.K, a[u][1]);
         f[u] = __ldg(sw + kb);
     };
     #pragma unroll
-    for (int u = 0; u < DEPTH; ++u) load_w(u, warp + u * S_WARPS);
+    for (int u = 0; u < DEPTH; ++u) load_w(u, kb0 + u);
     wait_for_previous_launch();
-    for (int kb = warp; kb < nkb; kb += DEPTH * S_WARPS)
+    for (int kb = kb0; kb < kb1; kb += DEPTH)
     {
         #pragma unroll
         for (int u = 0; u < DEPTH; ++u)
         {
-            const int k = kb + u * S_WARPS;
-            if (k >= nkb) break;
+            const int k = kb + u;
+            if (k >= kb1) break;
             #pragma unroll
             for (int j = 0; j < NG; ++j)
             {
@@ -285,7 +289,7 @@ void linear_tokens_kernel(const SmallLinearArgs p)
                 acc[j][2] = fmaf(c[2], f0, acc[j][2]);
                 acc[j][3] = fmaf(c[3], f1, acc[j][3]);
             }
-            load_w(u, k + DEPTH * S_WARPS);
+            load_w(u, k + DEPTH);
         }
     }
     #pragma unroll
@@ -304,7 +308,7 @@ void linear_tokens_kernel(const SmallLinearArgs p)
         {
             float v = 0.0f;
             #pragma unroll
-            for (int w = 0; w < S_WARPS; ++w) v += s_sum[w][threadIdx.x & 15][m];
+            for (int w = 0; w < T_WARPS; ++w) v += s_sum[w][threadIdx.x & 15][m];
             put(p.out, p.out_dtype, m * p.out_stride + n, v, p.accumulate != 0);
         }
     }
@@ -338,7 +342,7 @@ __device__ __forceinline__ float weight_of(const SmallExpertArgs& p, int64_t slo
 
 // Gate and up rows n0 .. n0 + 15 of the expert of route blockIdx.y: act = silu(min(g, L)) * clamp(u, -L, L), fp32.
 template <class T>
-__global__ __launch_bounds__(S_THREADS, 2)
+__global__ __launch_bounds__(S_THREADS, 3)
 void gate_up_token_kernel(const SmallExpertArgs p)
 {
     __shared__ float s_sum[S_WARPS][32];
@@ -379,15 +383,15 @@ void gate_up_token_kernel(const SmallExpertArgs p)
 
 // Output columns n0 .. n0 + 15 of token blockIdx.y: the activations quantised on the way, every route's product, and their
 // weighted sum in slot order.  The (route, part of K) units of a token are dealt to the warps.
-__global__ __launch_bounds__(S_THREADS, 2)
+__global__ __launch_bounds__(T_THREADS, 2)
 void down_token_kernel(const SmallExpertArgs p)
 {
     __shared__ float s_sum[32][16];                                 // [unit][row]: topk * parts units, at most 32
     const int64_t t = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int n0 = blockIdx.x * 16, nkb = p.f / kBlock;
-    const int parts = p.topk < S_WARPS ? (S_WARPS + p.topk - 1) / p.topk : 1;
-    for (int u = warp; u < p.topk * parts; u += S_WARPS)
+    const int parts = (T_WARPS + p.topk - 1) / p.topk;
+    for (int u = warp; u < p.topk * parts; u += T_WARPS)
     {
         const int64_t slot = t * p.topk + u / parts;
         const int64_t e = route_expert(p, slot);
@@ -396,7 +400,7 @@ void down_token_kernel(const SmallExpertArgs p)
         const uint8_t* const row[1][2] = {{w + (int64_t) (n0 + g) * p.f, w + (int64_t) (n0 + g + 8) * p.f}};
         const float* const sw[1] = {p.s2 + (e * (p.d / kBlock) + n0 / kBlock) * nkb};
         float acc[1][2];
-        stream_token<1, 4, true>(row, sw, p.act + slot * p.f, true, p.f, u % parts * nkb / parts,
+        stream_token<1, 1, true>(row, sw, p.act + slot * p.f, true, p.f, u % parts * nkb / parts,
                                    (u % parts + 1) * nkb / parts, 1, lane, acc);
         if ((lane & 3) == 0)
         {
@@ -428,7 +432,7 @@ int launch_dependent(void (*kernel)(Args), dim3 grid, cudaStream_t stream, const
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(S_THREADS);
+    cfg.blockDim = dim3(T_THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -454,8 +458,8 @@ int launch_fp8_linear_token(const void* x, int dtype, int K, const void* w, int6
     const unsigned grid = (unsigned) ((N + 15) / 16);
     auto go = [&](auto v) {
         using T = decltype(v);
-        if (a32) linear_token_kernel<true, T><<<grid, S_THREADS, 0, stream>>>(p);
-        else linear_token_kernel<false, T><<<grid, S_THREADS, 0, stream>>>(p);
+        if (a32) linear_token_kernel<true, T><<<grid, T_THREADS, 0, stream>>>(p);
+        else linear_token_kernel<false, T><<<grid, T_THREADS, 0, stream>>>(p);
     };
     if (dtype == 0) go(float{});
     else if (dtype == 1) go(__half{});
