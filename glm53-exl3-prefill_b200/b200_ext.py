@@ -15,6 +15,7 @@ library is missing the import of this module's loader fails loudly.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -367,141 +368,176 @@ def combine_slots(y, ids, n_experts, out, accumulate=False):
 
 
 # ------------------------------------------------------------------------------------ routing from logits, 8-bit layers
-# No reference counterpart.
+# No reference counterpart.  A decode step makes these calls for a few microseconds of GPU work each, so the checks
+# read plain attributes, messages are built only on failure, and the device guard is entered only for tensors of
+# another device than the current one.
 _DTYPE_NAMES = "float32, float16 or bfloat16"
+_E4M3 = torch.float8_e4m3fn
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
+               or (lambda index: torch.cuda.current_stream(index).cuda_stream))
 
 
-def _check_rows(x, what):
-    _check(x.dtype in _WDTYPE, f"{what} must be {_DTYPE_NAMES}")
-    _check(x.dim() == 2 and (x.size(1) <= 1 or x.stride(1) == 1) and (x.size(0) <= 1 or x.stride(0) >= x.size(1)),
-           f"{what} must be [rows, columns] with contiguous, separate rows")
+def _launch(index, fn, *args):
+    """fn(*args, stream) on GPU `index` and its current stream."""
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        raise RuntimeError(load().exl3_last_error().decode(errors="replace"))
 
 
-def _same_device(dev, *ts):
-    _check(all(t is None or t.device == dev for t in ts), "tensors must be on one device")
+def _status_ptr(index):
+    return status_tensor(torch.device("cuda", index)).data_ptr()
+
+
+def _fail(msg):
+    raise RuntimeError(msg)
+
+
+def _gpu_of(first, *others):
+    """The GPU that all tensors are on."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _fail("tensors must be CUDA" if index < 0 or t.get_device() < 0 else "tensors must be on one device")
+    if index < 0:
+        _fail("tensors must be CUDA")
+    return index
+
+
+def _rows_of(x, what):
+    """(rows, columns, row stride) of a 2-D tensor with contiguous, separate rows of a dtype the kernels read."""
+    if x.dtype not in _WDTYPE:
+        _fail(f"{what} must be {_DTYPE_NAMES}")
+    if x.dim() != 2:
+        _fail(f"{what} must be [rows, columns]")
+    rows, cols = x.shape
+    stride, one = x.stride()
+    if (cols > 1 and one != 1) or (rows > 1 and stride < cols):
+        _fail(f"{what} must be [rows, columns] with contiguous, separate rows")
+    return rows, cols, stride
+
+
+def _check_out(out, T, N, what):
+    if (out.dtype not in _WDTYPE or out.dim() != 2 or out.shape[0] != T or out.shape[1] != N
+            or (N > 1 and out.stride(1) != 1)):
+        _fail(f"{what}: out [{T}, {N}] ({_DTYPE_NAMES}, contiguous rows) on the input's device")
 
 
 def route_logits(logits, bias, topk, softmax, n_group, topk_group, group_top, norm, scale, ids, weights):
     """exl3_route_logits: logits [T, E] -> ids int64 / weights fp32 [T, topk]."""
-    _check_rows(logits, "route_logits: logits")
-    T, E = int(logits.size(0)), int(logits.size(1))
-    _check(bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.numel() == E),
-           "route_logits: bias fp32 [E]")
-    _check(ids.dtype == torch.int64 and ids.is_contiguous() and tuple(ids.shape) == (T, topk),
-           "route_logits: ids int64 [T, topk]")
-    _check(weights.dtype == torch.float32 and weights.is_contiguous() and tuple(weights.shape) == (T, topk),
-           "route_logits: weights fp32 [T, topk]")
-    _cuda(logits, bias, ids, weights)
-    _same_device(logits.device, bias, ids, weights)
-    lib = load()
-    with torch.cuda.device(logits.device):
-        _call(lib.exl3_route_logits, _ptr(logits), _WDTYPE[logits.dtype], T, E, logits.stride(0), _ptr(bias),
-              1 if softmax else 0, int(n_group), int(topk_group), int(group_top), int(topk), 1 if norm else 0,
-              float(scale), _ptr(ids), _ptr(weights), _stream(logits.device))
+    T, E, stride = _rows_of(logits, "route_logits: logits")
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous() or bias.numel() != E):
+        _fail("route_logits: bias fp32 [E]")
+    if ids.dtype != torch.int64 or not ids.is_contiguous() or ids.shape != (T, topk):
+        _fail("route_logits: ids int64 [T, topk]")
+    if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (T, topk):
+        _fail("route_logits: weights fp32 [T, topk]")
+    index = _gpu_of(logits, bias, ids, weights)
+    _launch(index, load().exl3_route_logits, logits.data_ptr(), _WDTYPE[logits.dtype], T, E, stride,
+            None if bias is None else bias.data_ptr(), 1 if softmax else 0, n_group, topk_group, group_top, topk,
+            1 if norm else 0, scale, ids.data_ptr(), weights.data_ptr())
 
 
 def fp8_quantize_rows(x, pow2, q, scale):
     """exl3_fp8_quantize_rows: x [T, K] -> q e4m3 [T, K], scale fp32 [T, ceil(K / 128)] (any strides)."""
-    _check_rows(x, "fp8_quantize_rows: x")
-    T, K = int(x.size(0)), int(x.size(1))
-    _check(q.dtype == torch.float8_e4m3fn and tuple(q.shape) == (T, K) and (K <= 1 or q.stride(1) == 1),
-           "fp8_quantize_rows: q e4m3 [T, K]")
-    _check(scale.dtype == torch.float32 and tuple(scale.shape) == (T, -(-K // 128)),
-           "fp8_quantize_rows: scale fp32 [T, ceil(K / 128)]")
-    _cuda(x, q, scale)
-    _same_device(x.device, q, scale)
-    lib = load()
-    with torch.cuda.device(x.device):
-        _call(lib.exl3_fp8_quantize_rows, _ptr(x), _WDTYPE[x.dtype], T, K, x.stride(0), 1 if pow2 else 0, _ptr(q),
-              q.stride(0), _ptr(scale), scale.stride(0), scale.stride(1), _stream(x.device))
+    T, K, stride = _rows_of(x, "fp8_quantize_rows: x")
+    if q.dtype != _E4M3 or q.shape != (T, K) or (K > 1 and q.stride(1) != 1):
+        _fail("fp8_quantize_rows: q e4m3 [T, K]")
+    if scale.dtype != torch.float32 or scale.shape != (T, -(-K // 128)):
+        _fail("fp8_quantize_rows: scale fp32 [T, ceil(K / 128)]")
+    index = _gpu_of(x, q, scale)
+    s_row, s_blk = scale.stride()
+    _launch(index, load().exl3_fp8_quantize_rows, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, 1 if pow2 else 0,
+            q.data_ptr(), q.stride(0), scale.data_ptr(), s_row, s_blk)
 
 
-def _check_out(out, T, N, dev, what):
-    _check(out.dtype in _WDTYPE and tuple(out.shape) == (T, N) and (N <= 1 or out.stride(1) == 1) and out.device == dev,
-           f"{what}: out [{T}, {N}] ({_DTYPE_NAMES}, contiguous rows) on the input's device")
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name, *sizes):
+    n = int(getattr(load(), name)(*sizes))
+    if n < 0:
+        _fail(load().exl3_last_error().decode(errors="replace") or f"{name}: invalid sizes")
+    return n
+
+
+def _workspace(index, name, *sizes):
+    """(tensor, address, bytes) of the scratch a call needs, from torch's caching allocator."""
+    n = _workspace_bytes(name, *sizes)
+    if n == 0:
+        return None, None, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", index))
+    return ws, ws.data_ptr(), n
 
 
 def fp8_linear(x, w, w_scale, out, accumulate=False):
     """exl3_fp8_linear: out [T, N] (+)= quantised(x [T, K]) . w^T, w e4m3 [N, K], w_scale fp32 [N/128, K/128]."""
-    _check_rows(x, "fp8_linear: x")
-    T, K = int(x.size(0)), int(x.size(1))
-    _check(w.dtype == torch.float8_e4m3fn and w.dim() == 2 and w.size(1) == K and (K <= 1 or w.stride(1) == 1),
-           "fp8_linear: weight e4m3 [N, K] with contiguous rows")
-    N = int(w.size(0))
-    _check(w_scale.dtype == torch.float32 and tuple(w_scale.shape) == (-(-N // 128), -(-K // 128))
-           and (w_scale.size(1) <= 1 or w_scale.stride(1) == 1), "fp8_linear: weight_scale fp32 [ceil(N/128), ceil(K/128)]")
-    _cuda(x, w, w_scale, out)
-    _check_out(out, T, N, x.device, "fp8_linear")
-    _same_device(x.device, w, w_scale)
-    lib = load()
-    need = int(lib.exl3_fp8_linear_workspace(T, K))
-    _check(need >= 0, "fp8_linear: K must be a multiple of 16")
-    dev = x.device
-    with torch.cuda.device(dev):
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _call(lib.exl3_fp8_linear, _ptr(x), _WDTYPE[x.dtype], T, K, x.stride(0), _ptr(w), w.stride(0), _ptr(w_scale),
-              max(w_scale.stride(0), w_scale.size(1)), N, _ptr(out), _WDTYPE[out.dtype], out.stride(0),
-              1 if accumulate else 0, _ptr(ws), need, _ptr(status_tensor(dev)), _stream(dev))
+    T, K, stride = _rows_of(x, "fp8_linear: x")
+    if w.dtype != _E4M3 or w.dim() != 2 or w.shape[1] != K or (K > 1 and w.stride(1) != 1):
+        _fail("fp8_linear: weight e4m3 [N, K] with contiguous rows")
+    N, kb = w.shape[0], -(-K // 128)
+    if w_scale.dtype != torch.float32 or w_scale.shape != (-(-N // 128), kb) or (kb > 1 and w_scale.stride(1) != 1):
+        _fail("fp8_linear: weight_scale fp32 [ceil(N/128), ceil(K/128)]")
+    index = _gpu_of(x, w, w_scale, out)
+    _check_out(out, T, N, "fp8_linear")
+    if K % 16:
+        _fail("fp8_linear: K must be a multiple of 16")
+    ws, ptr, nbytes = _workspace(index, "exl3_fp8_linear_workspace", T, K)
+    _launch(index, load().exl3_fp8_linear, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, w.data_ptr(), w.stride(0),
+            w_scale.data_ptr(), max(w_scale.stride(0), kb), N, out.data_ptr(), _WDTYPE[out.dtype], out.stride(0),
+            1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
 
 
 def _check_fp8_layer(w13, s13, w2, s2, d, what):
-    _check(w13.dtype == torch.float8_e4m3fn and w13.dim() == 3 and w13.size(2) == d and w13.size(1) % 256 == 0
-           and w13.is_contiguous(), f"{what}: w13_fp8 e4m3 [E, 2f, d], f a multiple of 128")
-    E, f = int(w13.size(0)), int(w13.size(1)) // 2
-    _check(d % 128 == 0, f"{what}: d must be a multiple of 128")
-    _check(w2.dtype == torch.float8_e4m3fn and tuple(w2.shape) == (E, d, f) and w2.is_contiguous(),
-           f"{what}: w2_fp8 e4m3 [E, d, f]")
-    _check(s13.dtype == torch.float32 and tuple(s13.shape) == (E, 2 * f // 128, d // 128) and s13.is_contiguous(),
-           f"{what}: w13_scale fp32 [E, 2f/128, d/128]")
-    _check(s2.dtype == torch.float32 and tuple(s2.shape) == (E, d // 128, f // 128) and s2.is_contiguous(),
-           f"{what}: w2_scale fp32 [E, d/128, f/128]")
-    _cuda(w13, s13, w2, s2)
+    if w13.dtype != _E4M3 or w13.dim() != 3 or w13.shape[2] != d or w13.shape[1] % 256 or not w13.is_contiguous():
+        _fail(f"{what}: w13_fp8 e4m3 [E, 2f, d], f a multiple of 128")
+    E, f = w13.shape[0], w13.shape[1] // 2
+    if d % 128:
+        _fail(f"{what}: d must be a multiple of 128")
+    if w2.dtype != _E4M3 or w2.shape != (E, d, f) or not w2.is_contiguous():
+        _fail(f"{what}: w2_fp8 e4m3 [E, d, f]")
+    if s13.dtype != torch.float32 or s13.shape != (E, f // 64, d // 128) or not s13.is_contiguous():
+        _fail(f"{what}: w13_scale fp32 [E, 2f/128, d/128]")
+    if s2.dtype != torch.float32 or s2.shape != (E, d // 128, f // 128) or not s2.is_contiguous():
+        _fail(f"{what}: w2_scale fp32 [E, d/128, f/128]")
     return E, f
 
 
 def fp8_mlp(x, w13, w13_scale, w2, w2_scale, limit, out, accumulate=False):
     """exl3_fp8_mlp: out [T, d] (+)= the gated MLP stored as one expert ([1, 2f, d], [1, d, f]) of x [T, d]."""
-    _check_rows(x, "fp8_mlp: x")
-    T, d = int(x.size(0)), int(x.size(1))
+    T, d, stride = _rows_of(x, "fp8_mlp: x")
     E, f = _check_fp8_layer(w13, w13_scale, w2, w2_scale, d, "fp8_mlp")
-    _check(E == 1, "fp8_mlp: the MLP must be stored as one expert ([1, ...] tensors)")
-    _cuda(x, out)
-    _check_out(out, T, d, x.device, "fp8_mlp")
-    _same_device(x.device, w13, w13_scale, w2, w2_scale)
-    lib = load()
-    dev = x.device
-    need = int(lib.exl3_fp8_mlp_workspace(T, d, f))
-    with torch.cuda.device(dev):
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _call(lib.exl3_fp8_mlp, _ptr(x), _WDTYPE[x.dtype], T, d, x.stride(0), _ptr(w13), _ptr(w13_scale), _ptr(w2),
-              _ptr(w2_scale), f, float(limit), _ptr(out), _WDTYPE[out.dtype], out.stride(0), 1 if accumulate else 0,
-              _ptr(ws), need, _ptr(status_tensor(dev)), _stream(dev))
+    if E != 1:
+        _fail("fp8_mlp: the MLP must be stored as one expert ([1, ...] tensors)")
+    index = _gpu_of(x, w13, w13_scale, w2, w2_scale, out)
+    _check_out(out, T, d, "fp8_mlp")
+    ws, ptr, nbytes = _workspace(index, "exl3_fp8_mlp_workspace", T, d, f)
+    _launch(index, load().exl3_fp8_mlp, x.data_ptr(), _WDTYPE[x.dtype], T, d, stride, w13.data_ptr(),
+            w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), f, limit, out.data_ptr(), _WDTYPE[out.dtype],
+            out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
 
 
 def fp8_experts(x, ids, weights, w13, w13_scale, w2, w2_scale, limit, out, accumulate=False):
     """exl3_fp8_experts: out [T, d] (+)= sum_j weights[t, j] * mlp_{ids[t, j]}(x[t]) over e4m3 experts."""
-    _check_rows(x, "fp8_experts: x")
-    T, d = int(x.size(0)), int(x.size(1))
+    T, d, stride = _rows_of(x, "fp8_experts: x")
     E, f = _check_fp8_layer(w13, w13_scale, w2, w2_scale, d, "fp8_experts")
-    _check(ids.dtype in (torch.int64, torch.int32), "ids must be int64 or int32")
-    _check(weights.dtype in _WDTYPE, "weights must be float32, float16 or bfloat16")
-    _check(ids.dim() == 2 and ids.size(0) == T and ids.is_contiguous() and weights.is_contiguous()
-           and weights.shape == ids.shape, "ids / weights must be contiguous [T, topk]")
-    topk = int(ids.size(1))
-    _cuda(x, ids, weights, out)
-    _check_out(out, T, d, x.device, "fp8_experts")
-    _same_device(x.device, ids, weights, w13, w13_scale, w2, w2_scale)
-    lib = load()
-    dev = x.device
-    need = int(lib.exl3_fp8_experts_workspace(T, topk, E, d, f))
-    if need < 0:
-        raise RuntimeError(lib.exl3_last_error().decode(errors="replace"))
-    with torch.cuda.device(dev):
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _call(lib.exl3_fp8_experts, _ptr(x), _WDTYPE[x.dtype], T, d, x.stride(0), _ptr(ids),
-              1 if ids.dtype == torch.int64 else 0, _ptr(weights), _WDTYPE[weights.dtype], topk, E, _ptr(w13),
-              _ptr(w13_scale), _ptr(w2), _ptr(w2_scale), f, float(limit), _ptr(out), _WDTYPE[out.dtype], out.stride(0),
-              1 if accumulate else 0, _ptr(ws), need, _ptr(status_tensor(dev)), _stream(dev))
+    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
+        _fail("ids must be int64 or int32")
+    if weights.dtype not in _WDTYPE:
+        _fail(f"weights must be {_DTYPE_NAMES}")
+    if (ids.dim() != 2 or ids.shape[0] != T or not ids.is_contiguous() or not weights.is_contiguous()
+            or weights.shape != ids.shape):
+        _fail("ids / weights must be contiguous [T, topk]")
+    topk = ids.shape[1]
+    index = _gpu_of(x, ids, weights, w13, w13_scale, w2, w2_scale, out)
+    _check_out(out, T, d, "fp8_experts")
+    ws, ptr, nbytes = _workspace(index, "exl3_fp8_experts_workspace", T, topk, E, d, f)
+    _launch(index, load().exl3_fp8_experts, x.data_ptr(), _WDTYPE[x.dtype], T, d, stride, ids.data_ptr(),
+            1 if ids.dtype == torch.int64 else 0, weights.data_ptr(), _WDTYPE[weights.dtype], topk, E, w13.data_ptr(),
+            w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), f, limit, out.data_ptr(), _WDTYPE[out.dtype],
+            out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
 
 
 # ------------------------------------------------------------------------------------ expert parallelism

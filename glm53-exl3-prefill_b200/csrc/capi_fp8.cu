@@ -171,6 +171,7 @@ int exl3_fp8_quantize_rows(const void* x, int64_t dtype, int64_t rows, int64_t K
 int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K)
 {
     if (T < 0 || T > kMaxDim || K < 16 || K % 16 != 0 || K > (1 << 24)) return -1;
+    if (T <= 1) return 0;                               // one row is quantised on the way
     Carver c{nullptr};
     take_rows(c, T, K);
     return c.used;
@@ -187,7 +188,7 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     if (N < 1 || N > (1 << 24)) return set_error("fp8_linear: invalid number of weight rows");
     if (T == 0) return EXL3_OK;
     if ((rc = check_out("fp8_linear", out, out_dtype, T, N, out_stride))) return rc;
-    if (!x || !w || !w_scale || !workspace) return set_error("tensors must be CUDA");
+    if (!x || !w || !w_scale || (!workspace && T > 1)) return set_error("tensors must be CUDA");
     if (!aligned16(w) || w_stride % 16 != 0 || w_stride < K)
         return set_error("fp8_linear: the weight's rows must be 16-byte aligned");
     if (w_scale_stride < blocks128(K)) return set_error("fp8_linear: weight scales [ceil(N / 128), ceil(K / 128)]");

@@ -3,10 +3,11 @@
 // A warp takes 16 weight rows and streams them from global memory straight into the A fragments of
 // mma.sync m16n8k32 (e4m3, fp32 sums): lane (g, t) = (lane / 4, lane % 4) reads the 32 bytes t of a row's 128-byte K
 // block, for rows g and g + 8, and the K order inside a block is permuted alike for both operands, so a fragment
-// is what one 32-byte load brings.  No shared memory, no barrier before the sums; the K blocks of a row tile
-// are dealt to a CTA's eight warps, whose sums are added in a fixed order at the end.  The tensor pipe is idle most of
-// the time either way (one column in eight is used for one token); what counts is that the loads of all
-// resident warps (128 KB per SM) are in flight from the start, and that one launch does everything:
+// is what one 32-byte load brings.  No shared memory and no barrier before the sums; a row tile's K blocks are dealt in runs
+// to a CTA's warps, whose sums are added in a fixed order at the end.  What counts is the number of warps that wait for memory:
+// one block in flight in each of 32 warps per SM beats four in each of 16 (6.4 against 8.4 us for one token,
+// 4096 x 4096, whose bytes take 2.6 us); neither rows copied to shared memory by the bulk-copy engine nor fp16
+// products were faster.  One launch does everything:
 //   one token   rows are quantised on the way: a warp reads a block's 128 values (4 a lane), takes their maximum, rounds
 //               them, and hands the words to the lanes whose fragment they belong to;
 //   2..16       (linear) rows are quantised by their own kernel first and read as fragments from L2.
@@ -240,12 +241,12 @@ void linear_token_kernel(const SmallLinearArgs p)
 }
 
 // 2..16 tokens: NG groups of 8 columns.
-template <int NG, bool ALIGNED32>
-__global__ __launch_bounds__(T_THREADS, 2)
+template <int NG, int WARPS, bool ALIGNED32>
+__global__ __launch_bounds__(WARPS * 32, 2)
 void linear_tokens_kernel(const SmallLinearArgs p)
 {
-    constexpr int DEPTH = 1;
-    __shared__ float s_sum[T_WARPS][16][NG * 8];
+    constexpr int DEPTH = NG;                              // blocks of weights in flight per warp
+    __shared__ float s_sum[WARPS][16][NG * 8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * 16, g = lane >> 2, t = lane & 3;
     const int nkb = (p.K + kBlock - 1) / kBlock;
@@ -255,7 +256,7 @@ void linear_tokens_kernel(const SmallLinearArgs p)
     float acc[NG][4];
     #pragma unroll
     for (int j = 0; j < NG; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-    const int kb0 = warp * nkb / T_WARPS, kb1 = (warp + 1) * nkb / T_WARPS;
+    const int kb0 = warp * nkb / WARPS, kb1 = (warp + 1) * nkb / WARPS;
     uint32_t a[DEPTH][2][8];
     float f[DEPTH];
     auto load_w = [&](int u, int kb) {
@@ -308,7 +309,7 @@ void linear_tokens_kernel(const SmallLinearArgs p)
         {
             float v = 0.0f;
             #pragma unroll
-            for (int w = 0; w < T_WARPS; ++w) v += s_sum[w][threadIdx.x & 15][m];
+            for (int w = 0; w < WARPS; ++w) v += s_sum[w][threadIdx.x & 15][m];
             put(p.out, p.out_dtype, m * p.out_stride + n, v, p.accumulate != 0);
         }
     }
@@ -428,11 +429,11 @@ void down_token_kernel(const SmallExpertArgs p)
 
 // A launch that may start before the one in front of it on the stream has ended (its kernel waits for that itself).
 template <class Args>
-int launch_dependent(void (*kernel)(Args), dim3 grid, cudaStream_t stream, const Args& args, const char* what)
+int launch_dependent(void (*kernel)(Args), dim3 grid, int threads, cudaStream_t stream, const Args& args, const char* what)
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(T_THREADS);
+    cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -477,12 +478,13 @@ int launch_fp8_linear_tokens(const Fp8GemmProblem& q, cudaStream_t stream)
     const bool a32 = reinterpret_cast<uintptr_t>(q.w) % 32 == 0 && q.w_stride % 32 == 0 &&
                      reinterpret_cast<uintptr_t>(q.x) % 32 == 0 && q.x_stride % 32 == 0;
     const unsigned grid = (unsigned) ((q.N + 15) / 16);
+    // two groups of columns need twice the registers, so half the warps with twice the blocks in flight
     const char* what = "fp8_linear (few tokens)";
     if (q.rows <= 8)
-        return a32 ? launch_dependent(linear_tokens_kernel<1, true>, dim3(grid), stream, p, what)
-                   : launch_dependent(linear_tokens_kernel<1, false>, dim3(grid), stream, p, what);
-    return a32 ? launch_dependent(linear_tokens_kernel<2, true>, dim3(grid), stream, p, what)
-               : launch_dependent(linear_tokens_kernel<2, false>, dim3(grid), stream, p, what);
+        return a32 ? launch_dependent(linear_tokens_kernel<1, T_WARPS, true>, dim3(grid), T_THREADS, stream, p, what)
+                   : launch_dependent(linear_tokens_kernel<1, T_WARPS, false>, dim3(grid), T_THREADS, stream, p, what);
+    return a32 ? launch_dependent(linear_tokens_kernel<2, S_WARPS, true>, dim3(grid), S_THREADS, stream, p, what)
+               : launch_dependent(linear_tokens_kernel<2, S_WARPS, false>, dim3(grid), S_THREADS, stream, p, what);
 }
 
 int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_stride, const void* ids, int ids_i64,
@@ -504,7 +506,7 @@ int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_s
     else gate_up_token_kernel<__nv_bfloat16><<<grid, S_THREADS, 0, stream>>>(p);
     int rc = check_launch("fp8_experts (gate and up, few routes)");
     if (rc) return rc;
-    return launch_dependent(down_token_kernel, dim3((unsigned) (d / 16), (unsigned) T), stream, p,
+    return launch_dependent(down_token_kernel, dim3((unsigned) (d / 16), (unsigned) T), T_THREADS, stream, p,
                             "fp8_experts (down, few routes)");
 }
 
