@@ -389,8 +389,9 @@ def _launch(index, fn, *args):
         raise RuntimeError(load().exl3_last_error().decode(errors="replace"))
 
 
+@functools.lru_cache(maxsize=None)
 def _status_ptr(index):
-    return status_tensor(torch.device("cuda", index)).data_ptr()
+    return status_tensor(torch.device("cuda", index)).data_ptr()      # (the tensor stays for the process's life)
 
 
 def _fail(msg):

@@ -11,14 +11,16 @@
 // The sigmoid router of GLM-5.3-Flash (docs/research/02-glm-5.3-flash-architecture.md:33) is the case
 // of one group; router.cu fuses that case with the router's product for callers that hold hidden states.
 //
-// One warp per token: lane i holds experts i, i + 32, ... as keys (unsigned integers in the order of the
-// floats), and each of the topk rounds is two warp-wide integer reductions (the largest key, then the lowest
-// expert that holds it) and a rescan by the lane that owned it.
+// One warp per token: lane i holds experts i, i + 32, ... as keys (unsigned integers in the order of the floats) and
+// knows its two best; each of the topk rounds is two warp-wide integer reductions (the largest key, then the lowest
+// expert that holds it), after which the owner moves up its second best and only looks at its keys again when that is
+// gone too.  The bytes of the logits (33 MB for 32768 tokens of 256 experts, 5 us) bound it in principle; the instructions do
+// in fact, about 450 a token.
 //
 // The choice is the one that exact arithmetic makes.  Without a bias both score functions grow with the
-// logit, so experts are ranked by the logits themselves.  With a bias, or for sums of a group's best, the 32-bit
-// scores rank them, and wherever two scores that a decision separates are closer than 32-bit arithmetic
-// can tell (kTol), that token is decided again in 64 bits.
+// logit, so experts are ranked by the logits themselves.  With a bias, scores in 32 bits rank them, and where two scores
+// that a decision separates are closer than that arithmetic can tell (kTol), the candidates, one a lane, are
+// ranked again by their scores in 64 bits; where two groups nearly tie, the groups are.
 #include <cstdint>
 #include <type_traits>
 #include <cuda_bf16.h>
@@ -35,10 +37,11 @@ constexpr int RL_THREADS = 128;
 constexpr int RL_WARPS = RL_THREADS / 32;
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kNoExpert = 0x7fffffff;
-// Two selection scores closer than kTol * (1 + |c|) are not told apart in 32 bits.  A score's error: expf, a
-// sum and a division, under 2^-20 of a value that is at most 1, and the rounding of s + b, 2^-24 of it.
-// A sum of two doubles that; 8e-6 covers both.
-constexpr float kTol = 8e-6f;
+// Two selection scores closer than kTol * (1 + |c|) are not told apart in 32 bits.  A score's error: ex2.approx and
+// rcp.approx (2^-22 each, relative), the rounding of the exponent's argument (under 2^-24 * |l| s (1 - s) <= 2^-26), for softmax
+// the sum's (2^-20, relative): under 1.3e-6 of a value that is at most 1; and the rounding of s + b, 2^-24 of it.  Twice
+// that (two scores) is under 3e-6.
+constexpr float kTol = 4e-6f;
 
 struct RouteLogitsArgs {
     const void* logits;
@@ -88,29 +91,64 @@ __device__ __forceinline__ float warp_max(float v)
 // exp(l - m) of the softmax; the largest logit gives 1 even where it is +inf.
 __device__ __forceinline__ float soft_exp(float l, float m) { return l == m ? 1.0f : expf(l - m); }
 
-// The token's whole selection in 64 bits, by one warp: lane j < topk returns the expert of slot j (-1: none).
-// A rare path (a near-tie decides, kTol), written for its size: scores are computed again wherever needed.
-template <bool SOFTMAX, class Tl>
-__device__ __noinline__ int select_in_64_bits(const RouteLogitsArgs& p, const Tl* row, float m, int lane)
+// Scores for ranking: fast, to kTol.
+__device__ __forceinline__ float fast_exp(float l, float m) { return l == m ? 1.0f : __expf(l - m); }
+__device__ __forceinline__ float fast_sigmoid(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
+
+// The selection score of expert e in 64 bits (inv: the softmax's 1 / sum, in 64 bits).
+template <bool SOFTMAX>
+__device__ __forceinline__ double exact_score(const RouteLogitsArgs& p, float l, int e, float m, double inv)
 {
-    double inv = 1.0;
-    if (SOFTMAX)
+    const double s = SOFTMAX ? (l == m ? 1.0 : exp((double) l - (double) m)) * inv : 1.0 / (1.0 + exp(-(double) l));
+    return p.bias ? s + (double) p.bias[e] : s;
+}
+
+// The token's whole selection in 64 bits, by one warp: lane j < topk returns the expert of slot j (-1: none).  A path for
+// more than 32 candidates that nearly tie, written for its size: scores are computed again wherever needed.
+// 1 / sum of the softmax in 64 bits.
+template <class Tl>
+__device__ __forceinline__ double exact_inverse_sum(const RouteLogitsArgs& p, const Tl* row, float m, int lane)
+{
+    double z = 0.0;
+    for (int e = lane; e < p.E; e += 32)
     {
-        double z = 0.0;
-        for (int e = lane; e < p.E; e += 32)
-        {
-            const float l = load_logit(row + e);
-            if (l > -INFINITY) z += l == m ? 1.0 : exp((double) l - (double) m);
-        }
-        inv = 1.0 / warp_sum(z);
+        const float l = load_logit(row + e);
+        if (l > -INFINITY) z += l == m ? 1.0 : exp((double) l - (double) m);
     }
-    bool by_logit = false;                                  // the ranking without a bias
+    return 1.0 / warp_sum(z);
+}
+
+// The candidates, one per lane (expert mine, -1 past n of them; every other expert's score is clearly below the last
+// chosen one), ranked by their scores in 64 bits: lane j < topk returns the expert of slot j.
+template <bool SOFTMAX, class Tl>
+__device__ __noinline__ int rank_in_64_bits(const RouteLogitsArgs& p, const Tl* row, float m, int lane, int mine, int n)
+{
+    const double inv = SOFTMAX ? exact_inverse_sum(p, row, m, lane) : 1.0;
+    const double c = mine >= 0 ? exact_score<SOFTMAX>(p, load_logit(row + mine), mine, m, inv) : 0.0;
+    int rank = 0;
+    for (int j = 0; j < n; ++j)
+    {
+        const double o = __shfl_sync(kFull, c, j);
+        const int oe = __shfl_sync(kFull, mine, j);
+        rank += o > c || (o == c && oe < mine);
+    }
+    int out = -1;
+    for (int j = 0; j < n; ++j)
+    {
+        const int r = __shfl_sync(kFull, rank, j), e = __shfl_sync(kFull, mine, j);
+        if (r == lane) out = e;
+    }
+    return out;
+}
+
+template <bool SOFTMAX, class Tl>
+__device__ __noinline__ int select_in_64_bits(const RouteLogitsArgs& p, const Tl* row, float m, int lane, unsigned kept)
+{
+    const double inv = SOFTMAX ? exact_inverse_sum(p, row, m, lane) : 1.0;
     auto score = [&](int e, bool& ok) {
         const float l = load_logit(row + e);
         ok = l > -INFINITY;
-        if (by_logit) return (double) l;
-        const double s = SOFTMAX ? (l == m ? 1.0 : exp((double) l - (double) m)) * inv : 1.0 / (1.0 + exp(-(double) l));
-        return p.bias ? s + (double) p.bias[e] : s;
+        return exact_score<SOFTMAX>(p, l, e, m, inv);
     };
     // the best expert in [lo, hi) that comes after (pv, pe) in the order: larger score first, then lower number
     auto next = [&](int lo, int hi, unsigned groups, double pv, int pe, double& bv) {
@@ -132,33 +170,6 @@ __device__ __noinline__ int select_in_64_bits(const RouteLogitsArgs& p, const Tl
         }
         return be;
     };
-    unsigned kept = ~0u;
-    if (p.topk_group < p.n_group)
-    {
-        double gs = -INFINITY;                              // lane g: the score of group g
-        for (int g = 0; g < p.n_group; ++g)
-        {
-            double sum = 0.0, pv = 0.0;
-            int pe = -1;
-            for (int j = 0; j < p.group_top; ++j)
-            {
-                double v;
-                pe = next(g * p.per_group, (g + 1) * p.per_group, ~0u, pv, pe, v);
-                if (pe == kNoExpert) { sum = -INFINITY; break; }
-                pv = v;
-                sum += v;
-            }
-            if (lane == g) gs = sum;
-        }
-        int rank = 0;
-        for (int g = 0; g < p.n_group; ++g)
-        {
-            const double o = __shfl_sync(kFull, gs, g);
-            rank += o > gs || (o == gs && g < lane);
-        }
-        kept = __ballot_sync(kFull, lane < p.n_group && rank < p.topk_group);
-    }
-    by_logit = p.bias == nullptr;
     int mine = -1, pe = -1;
     double pv = 0.0;
     for (int j = 0; j < p.topk; ++j)
@@ -172,14 +183,75 @@ __device__ __noinline__ int select_in_64_bits(const RouteLogitsArgs& p, const Tl
     return mine;
 }
 
+template <class F> __device__ __forceinline__ F lowest();
+template <> __device__ __forceinline__ float lowest() { return -INFINITY; }
+template <> __device__ __forceinline__ double lowest() { return -(double) INFINITY; }
+
+// The groups kept (a bit each) by their scores, from the token's selection scores sc[E] in shared memory; `gap`: how far
+// the last kept group's score is above the best dropped one's, and `low` the former.  lanes_per_group lanes scan a group and
+// merge their two best.
+template <class F>
+__device__ __forceinline__ unsigned kept_groups(const RouteLogitsArgs& p, const F* sc, int lane, F& low, F& gap)
+{
+    const int lpg = p.lanes_per_group, g = lane / lpg, sub = lane - g * lpg;
+    F b1 = lowest<F>(), b2 = lowest<F>();
+    if (g < p.n_group)
+        for (int i = sub; i < p.per_group; i += lpg)
+        {
+            const F c = sc[g * p.per_group + i];
+            b2 = max(b2, min(b1, c));
+            b1 = max(b1, c);
+        }
+    for (int o = lpg >> 1; o > 0; o >>= 1)
+    {
+        const F o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+        b2 = max(min(b1, o1), max(b2, o2));
+        b1 = max(b1, o1);
+    }
+    const F mine = g < p.n_group ? (p.group_top > 1 ? b1 + b2 : b1) : lowest<F>();
+    const F gs = __shfl_sync(kFull, mine, (lane * lpg) & 31);               // lane g: group g
+    int rank = 0;
+    for (int o = 0; o < p.n_group; ++o)
+    {
+        const F x = __shfl_sync(kFull, gs, o);
+        rank += x > gs || (x == gs && o < lane);
+    }
+    const bool is_group = lane < p.n_group;
+    const unsigned last = __ballot_sync(kFull, is_group && rank == p.topk_group - 1);
+    const unsigned next = __ballot_sync(kFull, is_group && rank == p.topk_group);
+    low = __shfl_sync(kFull, gs, __ffs(last) - 1);
+    gap = low - __shfl_sync(kFull, gs, __ffs(next) - 1);
+    return __ballot_sync(kFull, is_group && rank < p.topk_group);
+}
+
+// The same from scores in 64 bits, which replace sc.
+template <bool SOFTMAX, class Tl>
+__device__ __noinline__ unsigned kept_groups_in_64_bits(const RouteLogitsArgs& p, const Tl* row, float m, int lane, double* sc)
+{
+    const double inv = SOFTMAX ? exact_inverse_sum(p, row, m, lane) : 1.0;
+    __syncwarp();
+    for (int e = lane; e < p.E; e += 32)
+    {
+        const float l = load_logit(row + e);
+        sc[e] = l > -INFINITY ? exact_score<SOFTMAX>(p, l, e, m, inv) : lowest<double>();
+    }
+    __syncwarp();
+    double low, gap;
+    return kept_groups<double>(p, sc, lane, low, gap);
+}
+
 // Registers: MPL = the experts a lane holds, at least ceil(E / 32).
 template <int MPL, bool SOFTMAX, class Tl>
 __global__ __launch_bounds__(RL_THREADS)
 void route_logits_kernel(const RouteLogitsArgs p)
 {
-    extern __shared__ float s_rows[];                       // [RL_WARPS][E]: selection scores (group selection only)
+    extern __shared__ double s_rows[];                      // [RL_WARPS][E]: selection scores (group selection only)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool grouped = p.topk_group < p.n_group;
+    const bool by_score = p.bias != nullptr;                // keys: the selection score with a bias, else the logit
+    float bias[MPL];
+    #pragma unroll
+    for (int i = 0; i < MPL; ++i) bias[i] = by_score && lane + 32 * i < p.E ? __ldg(p.bias + lane + 32 * i) : 0.0f;
     for (int64_t t = (int64_t) blockIdx.x * RL_WARPS + warp; t < p.T; t += (int64_t) gridDim.x * RL_WARPS)
     {
         const Tl* row = reinterpret_cast<const Tl*>(p.logits) + t * p.row_stride;
@@ -201,28 +273,21 @@ void route_logits_kernel(const RouteLogitsArgs p)
             float z = 0.0f;
             #pragma unroll
             for (int i = 0; i < MPL; ++i)
-                if (v[i] == v[i]) z += soft_exp(v[i], m);
+                if (v[i] == v[i]) z += fast_exp(v[i], m);
             inv = 1.0f / warp_sum(z);
         }
-        // keys: by the selection score with a bias, by the logit without one
-        const bool by_score = p.bias != nullptr;
         uint32_t key[MPL];
         #pragma unroll
         for (int i = 0; i < MPL; ++i)
         {
             float c = v[i];
-            if (by_score && c == c)
-            {
-                const float s = SOFTMAX ? soft_exp(c, m) * inv : 1.0f / (1.0f + expf(-c));
-                c = s + __ldg(p.bias + lane + 32 * i);
-            }
-            key[i] = c == c ? order_key(c) : 0u;
+            if (by_score) c = (SOFTMAX ? fast_exp(c, m) * inv : fast_sigmoid(c)) + bias[i];
+            key[i] = v[i] == v[i] ? order_key(c) : 0u;
         }
-        bool near = false;
+        unsigned kept = ~0u;
         if (grouped)
         {
-            // lanes_per_group lanes scan a group's scores from shared memory and merge their two best
-            float* sc = s_rows + warp * p.E;
+            float* sc = reinterpret_cast<float*>(s_rows + warp * p.E);
             const bool sums = p.group_top > 1;
             #pragma unroll
             for (int i = 0; i < MPL; ++i)
@@ -230,80 +295,82 @@ void route_logits_kernel(const RouteLogitsArgs p)
                 const int e = lane + 32 * i;
                 if (e >= p.E) continue;
                 float c = key[i] ? key_value(key[i]) : -INFINITY;
-                if (!by_score && sums && key[i]) c = SOFTMAX ? soft_exp(c, m) * inv : 1.0f / (1.0f + expf(-c));
+                if (!by_score && sums && key[i]) c = SOFTMAX ? fast_exp(c, m) * inv : fast_sigmoid(c);
                 sc[e] = c;
             }
             __syncwarp();
-            const int lpg = p.lanes_per_group, g = lane / lpg, sub = lane - g * lpg;
-            float b1 = -INFINITY, b2 = -INFINITY;
-            if (g < p.n_group)
-                for (int i = sub; i < p.per_group; i += lpg)
-                {
-                    const float c = sc[g * p.per_group + i];
-                    b2 = fmaxf(b2, fminf(b1, c));
-                    b1 = fmaxf(b1, c);
-                }
-            for (int o = lpg >> 1; o > 0; o >>= 1)
-            {
-                const float o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
-                b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
-                b1 = fmaxf(b1, o1);
-            }
-            const float mine = g < p.n_group ? (sums ? b1 + b2 : b1) : -INFINITY;
-            const float gs = __shfl_sync(kFull, mine, (lane * lpg) & 31);   // lane g: group g
-            int rank = 0;
-            for (int o = 0; o < p.n_group; ++o)
-            {
-                const float x = __shfl_sync(kFull, gs, o);
-                rank += x > gs || (x == gs && o < lane);
-            }
-            const bool in = lane < p.n_group && rank < p.topk_group;
-            const unsigned kept = __ballot_sync(kFull, in);
-            if (by_score || sums)
-            {
-                const float low = -warp_max(in ? -gs : -INFINITY);          // the last kept and the best dropped
-                const float high = warp_max(lane < p.n_group && !in ? gs : -INFINITY);
-                near = low - high <= 2.0f * kTol * (1.0f + fabsf(low)) && high > -INFINITY;
-            }
+            float low, gap;
+            kept = kept_groups<float>(p, sc, lane, low, gap);
+            // a group's score is a sum of up to two: twice the error of one.  (A group without two experts left is at
+            // -inf, and a gap of nothing to -inf is no near-tie.)
+            if ((by_score || sums) && gap <= 2.0f * kTol * (1.0f + fabsf(low)) && low > -INFINITY)
+                kept = kept_groups_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, s_rows + warp * p.E);
             #pragma unroll
             for (int i = 0; i < MPL; ++i)
                 if (!((kept >> min((lane + 32 * i) / p.per_group, 31)) & 1u)) key[i] = 0u;
             __syncwarp();                                                    // the row is rewritten for the next token
         }
-        // the lane's best: keys are compared in rising expert order, so equal keys leave the lowest expert
-        uint32_t lk = 0u;
-        int le = kNoExpert;
-        #pragma unroll
-        for (int i = 0; i < MPL; ++i)
-            if (key[i] > lk) { lk = key[i]; le = lane + 32 * i; }
         int my_id = -1;
-        float last = INFINITY;
-        const int rounds = by_score && !near ? p.topk + 1 : p.topk;          // one more: the best that is not chosen
-        for (int j = 0; j < rounds; ++j)
         {
-            const uint32_t best = __reduce_max_sync(kFull, lk);
-            if (best == 0u) break;
-            const int id = __reduce_min_sync(kFull, lk == best ? le : kNoExpert);
-            if (by_score)
+            // the lane's two best; keys are compared in rising expert order, so equal keys leave the lower expert first
+            uint32_t k1 = 0u, k2 = 0u;
+            int i1 = kNoExpert, i2 = kNoExpert;
+            #pragma unroll
+            for (int i = 0; i < MPL; ++i)
             {
-                const float c = key_value(best);
-                near |= j > 0 && last - c <= kTol * (1.0f + fabsf(c));
-                last = c;
+                const bool first = key[i] > k1, second = key[i] > k2;
+                k2 = first ? k1 : second ? key[i] : k2;
+                i2 = first ? i1 : second ? lane + 32 * i : i2;
+                k1 = first ? key[i] : k1;
+                i1 = first ? lane + 32 * i : i1;
             }
-            if (lane == j && j < p.topk) my_id = id;
-            if (le == id)
+            float last = 0.0f, floor_c = 0.0f;              // the score before this one; that of the last slot
+            bool ties = false;
+            int n = 0;                                      // candidates: topk, and what may belong before the last of them
+            for (; n < 32; ++n)
             {
-                lk = 0u;
-                le = kNoExpert;
-                #pragma unroll
-                for (int i = 0; i < MPL; ++i)
+                if (n >= p.topk && !by_score) break;
+                const uint32_t best = __reduce_max_sync(kFull, k1);
+                if (best == 0u) break;
+                if (by_score)
                 {
-                    if (lane + 32 * i == id) key[i] = 0u;
-                    if (key[i] > lk) { lk = key[i]; le = lane + 32 * i; }
+                    const float c = key_value(best), tol = kTol * (1.0f + fabsf(c));
+                    if (n >= p.topk)
+                    {
+                        if (floor_c - c > tol) break;
+                        ties = true;
+                    }
+                    else
+                    {
+                        ties |= n > 0 && last - c <= tol;
+                        floor_c = c;
+                    }
+                    last = c;
+                }
+                const int id = __reduce_min_sync(kFull, k1 == best ? i1 : kNoExpert);
+                if (lane == n) my_id = id;
+                if (i1 == id)
+                {
+                    if (k2 == 0u)                           // both known ones are gone: the best that comes after
+                    {
+                        #pragma unroll
+                        for (int i = 0; i < MPL; ++i)
+                        {
+                            const int e = lane + 32 * i;
+                            const bool after = key[i] < best || (key[i] == best && e > id);
+                            if (after && key[i] > k2) { k2 = key[i]; i2 = e; }
+                        }
+                    }
+                    k1 = k2;
+                    i1 = i2;
+                    k2 = 0u;
+                    i2 = kNoExpert;
                 }
             }
+            if (n == 32 && ties) my_id = select_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, kept);
+            else if (ties) my_id = rank_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, my_id, n);
+            if (lane >= p.topk) my_id = -1;
         }
-        if (near) my_id = select_in_64_bits<SOFTMAX, Tl>(p, row, m, lane);
         float s = 0.0f;
         if (my_id >= 0)
         {
@@ -340,8 +407,9 @@ int launch_route_logits(const void* logits, int dtype, int64_t T, int E, int64_t
     while (2 * p.lanes_per_group * n_group <= 32) p.lanes_per_group *= 2;
     p.norm = norm; p.scale = scale; p.ids = ids; p.weights = weights;
     const int64_t want = (T + RL_WARPS - 1) / RL_WARPS;
-    const unsigned grid = (unsigned) (want < (1 << 20) ? want : (1 << 20));
-    const size_t smem = topk_group < n_group ? sizeof(float) * RL_WARPS * (size_t) E : 0;
+    const int64_t most = (int64_t) device_sm_count() * 12;              // 48 warps an SM, each keeping its biases
+    const unsigned grid = (unsigned) (want < most ? want : most);
+    const size_t smem = topk_group < n_group ? sizeof(double) * RL_WARPS * (size_t) E : 0;
     // the smallest instantiation that holds ceil(E / 32) experts a lane
     auto go = [&](auto sm) {
         constexpr bool SM = decltype(sm)::value;
