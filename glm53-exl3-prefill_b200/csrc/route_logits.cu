@@ -91,9 +91,21 @@ __device__ __forceinline__ float warp_max(float v)
 // exp(l - m) of the softmax; the largest logit gives 1 even where it is +inf.
 __device__ __forceinline__ float soft_exp(float l, float m) { return l == m ? 1.0f : expf(l - m); }
 
-// Scores for ranking: fast, to kTol.
-__device__ __forceinline__ float fast_exp(float l, float m) { return l == m ? 1.0f : __expf(l - m); }
-__device__ __forceinline__ float fast_sigmoid(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
+// Scores for ranking: fast, to kTol (results below 2^-126 are zero, which is far below it).
+__device__ __forceinline__ float fast_exp2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+constexpr float kLog2e = 1.44269504f;
+__device__ __forceinline__ float fast_exp(float l, float m) { return l == m ? 1.0f : fast_exp2((l - m) * kLog2e); }
+__device__ __forceinline__ float fast_sigmoid(float l)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + fast_exp2(l * -kLog2e)));
+    return r;
+}
 
 // The selection score of expert e in 64 bits (inv: the softmax's 1 / sum, in 64 bits).
 template <bool SOFTMAX>
@@ -240,18 +252,27 @@ __device__ __noinline__ unsigned kept_groups_in_64_bits(const RouteLogitsArgs& p
     return kept_groups<double>(p, sc, lane, low, gap);
 }
 
+// CTAs that an SM holds at a time (64, 80 or 128 registers a thread).
+constexpr int rl_resident(int MPL) { return MPL <= 9 ? 8 : MPL <= 16 ? 6 : 4; }
+
 // Registers: MPL = the experts a lane holds, at least ceil(E / 32).
 template <int MPL, bool SOFTMAX, class Tl>
-__global__ __launch_bounds__(RL_THREADS)
-void route_logits_kernel(const RouteLogitsArgs p)
+__global__ __launch_bounds__(RL_THREADS, rl_resident(MPL))
+void route_logits_kernel(const __grid_constant__ RouteLogitsArgs p)
 {
     extern __shared__ double s_rows[];                      // [RL_WARPS][E]: selection scores (group selection only)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool grouped = p.topk_group < p.n_group;
     const bool by_score = p.bias != nullptr;                // keys: the selection score with a bias, else the logit
     float bias[MPL];
+    uint32_t group[MPL];                                    // the group's bit
     #pragma unroll
-    for (int i = 0; i < MPL; ++i) bias[i] = by_score && lane + 32 * i < p.E ? __ldg(p.bias + lane + 32 * i) : 0.0f;
+    for (int i = 0; i < MPL; ++i)
+    {
+        const int e = lane + 32 * i;
+        bias[i] = by_score && e < p.E ? __ldg(p.bias + e) : 0.0f;
+        group[i] = e < p.E ? 1u << (e / p.per_group) : 0u;
+    }
     for (int64_t t = (int64_t) blockIdx.x * RL_WARPS + warp; t < p.T; t += (int64_t) gridDim.x * RL_WARPS)
     {
         const Tl* row = reinterpret_cast<const Tl*>(p.logits) + t * p.row_stride;
@@ -307,7 +328,7 @@ void route_logits_kernel(const RouteLogitsArgs p)
                 kept = kept_groups_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, s_rows + warp * p.E);
             #pragma unroll
             for (int i = 0; i < MPL; ++i)
-                if (!((kept >> min((lane + 32 * i) / p.per_group, 31)) & 1u)) key[i] = 0u;
+                if (!(kept & group[i])) key[i] = 0u;
             __syncwarp();                                                    // the row is rewritten for the next token
         }
         int my_id = -1;
@@ -324,32 +345,16 @@ void route_logits_kernel(const RouteLogitsArgs p)
                 k1 = first ? key[i] : k1;
                 i1 = first ? lane + 32 * i : i1;
             }
-            float last = 0.0f, floor_c = 0.0f;              // the score before this one; that of the last slot
-            bool ties = false;
-            int n = 0;                                      // candidates: topk, and what may belong before the last of them
-            for (; n < 32; ++n)
-            {
-                if (n >= p.topk && !by_score) break;
+            uint32_t my_key = 0u;                           // lane n: the n-th best
+            auto take = [&](int n) {
                 const uint32_t best = __reduce_max_sync(kFull, k1);
-                if (best == 0u) break;
-                if (by_score)
-                {
-                    const float c = key_value(best), tol = kTol * (1.0f + fabsf(c));
-                    if (n >= p.topk)
-                    {
-                        if (floor_c - c > tol) break;
-                        ties = true;
-                    }
-                    else
-                    {
-                        ties |= n > 0 && last - c <= tol;
-                        floor_c = c;
-                    }
-                    last = c;
-                }
                 const int id = __reduce_min_sync(kFull, k1 == best ? i1 : kNoExpert);
-                if (lane == n) my_id = id;
-                if (i1 == id)
+                if (lane == n)
+                {
+                    my_key = best;
+                    my_id = best ? id : -1;
+                }
+                if (i1 == id && best)
                 {
                     if (k2 == 0u)                           // both known ones are gone: the best that comes after
                     {
@@ -366,9 +371,34 @@ void route_logits_kernel(const RouteLogitsArgs p)
                     k2 = 0u;
                     i2 = kNoExpert;
                 }
+            };
+            const int k = p.topk;
+            for (int n = 0; n < k; ++n) take(n);
+            if (by_score)
+            {
+                // near-ties among the chosen, and of the last of them with what is left
+                const uint32_t left = __reduce_max_sync(kFull, k1);
+                const uint32_t below = __shfl_down_sync(kFull, my_key, 1);
+                const uint32_t next = lane == k - 1 ? left : below;
+                const float c = key_value(my_key), tol = kTol * (1.0f + fabsf(c));
+                const bool tie = lane < k && next && c - key_value(next) <= tol;
+                if (__any_sync(kFull, tie))
+                {
+                    const uint32_t last = __shfl_sync(kFull, my_key, k - 1);
+                    const float bar = key_value(last) - kTol * (1.0f + fabsf(key_value(last)));
+                    int n = k;                              // candidates: topk, and what may belong before the last of them
+                    bool more = true;
+                    for (;; ++n)
+                    {
+                        const uint32_t best = __reduce_max_sync(kFull, k1);
+                        more = best && last && key_value(best) >= bar;
+                        if (!more || n == 32) break;
+                        take(n);
+                    }
+                    my_id = more ? select_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, kept)
+                                 : rank_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, my_id, n);
+                }
             }
-            if (n == 32 && ties) my_id = select_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, kept);
-            else if (ties) my_id = rank_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, my_id, n);
             if (lane >= p.topk) my_id = -1;
         }
         float s = 0.0f;
@@ -387,8 +417,13 @@ void route_logits_kernel(const RouteLogitsArgs p)
 }
 
 template <int MPL, bool SOFTMAX>
-void launch_typed(const RouteLogitsArgs& p, int dtype, unsigned grid, size_t smem, cudaStream_t stream)
+void launch_typed(const RouteLogitsArgs& p, int dtype, size_t smem, cudaStream_t stream)
 {
+    // as many CTAs as run at one time, each warp with the same number of tokens (give or take one) and its biases
+    // in registers
+    const int64_t want = (p.T + RL_WARPS - 1) / RL_WARPS, most = (int64_t) device_sm_count() * rl_resident(MPL);
+    const int64_t rounds = (want + most - 1) / most;
+    const unsigned grid = (unsigned) ((want + rounds - 1) / rounds);
     if (dtype == 0) route_logits_kernel<MPL, SOFTMAX, float><<<grid, RL_THREADS, smem, stream>>>(p);
     else if (dtype == 1) route_logits_kernel<MPL, SOFTMAX, __half><<<grid, RL_THREADS, smem, stream>>>(p);
     else route_logits_kernel<MPL, SOFTMAX, __nv_bfloat16><<<grid, RL_THREADS, smem, stream>>>(p);
@@ -406,18 +441,16 @@ int launch_route_logits(const void* logits, int dtype, int64_t T, int E, int64_t
     p.lanes_per_group = 1;
     while (2 * p.lanes_per_group * n_group <= 32) p.lanes_per_group *= 2;
     p.norm = norm; p.scale = scale; p.ids = ids; p.weights = weights;
-    const int64_t want = (T + RL_WARPS - 1) / RL_WARPS;
-    const int64_t most = (int64_t) device_sm_count() * 12;              // 48 warps an SM, each keeping its biases
-    const unsigned grid = (unsigned) (want < most ? want : most);
     const size_t smem = topk_group < n_group ? sizeof(double) * RL_WARPS * (size_t) E : 0;
     // the smallest instantiation that holds ceil(E / 32) experts a lane
     auto go = [&](auto sm) {
         constexpr bool SM = decltype(sm)::value;
-        if (E <= 64) launch_typed<2, SM>(p, dtype, grid, smem, stream);
-        else if (E <= 128) launch_typed<4, SM>(p, dtype, grid, smem, stream);
-        else if (E <= 288) launch_typed<9, SM>(p, dtype, grid, smem, stream);
-        else if (E <= 512) launch_typed<16, SM>(p, dtype, grid, smem, stream);
-        else launch_typed<32, SM>(p, dtype, grid, smem, stream);
+        if (E <= 64) launch_typed<2, SM>(p, dtype, smem, stream);
+        else if (E <= 128) launch_typed<4, SM>(p, dtype, smem, stream);
+        else if (E <= 256) launch_typed<8, SM>(p, dtype, smem, stream);
+        else if (E <= 288) launch_typed<9, SM>(p, dtype, smem, stream);
+        else if (E <= 512) launch_typed<16, SM>(p, dtype, smem, stream);
+        else launch_typed<32, SM>(p, dtype, smem, stream);
     };
     if (softmax) go(std::true_type{});
     else go(std::false_type{});
