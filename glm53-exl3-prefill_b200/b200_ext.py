@@ -60,7 +60,7 @@ _SIGNATURES = {
     "exl3_fat_gemm_scatter": ([_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _I32, _P, _P], _I32),
     "exl3_route_logits": ([_P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _F64, _P, _P, _P], _I32),
     "exl3_fp8_quantize_rows": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P], _I32),
-    "exl3_fp8_linear_workspace": ([_I64, _I64], _I64),
+    "exl3_fp8_linear_workspace": ([_I64, _I64, _I64], _I64),
     "exl3_fp8_linear": ([_P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _P, _P],
                         _I32),
     "exl3_fp8_mlp_workspace": ([_I64, _I64, _I64], _I64),
@@ -485,7 +485,7 @@ def fp8_linear(x, w, w_scale, out, accumulate=False):
     _check_out(out, T, N, "fp8_linear")
     if K % 16:
         _fail("fp8_linear: K must be a multiple of 16")
-    ws, ptr, nbytes = _workspace(index, "exl3_fp8_linear_workspace", T, K)
+    ws, ptr, nbytes = _workspace(index, "exl3_fp8_linear_workspace", T, K, N)
     _launch(index, load().exl3_fp8_linear, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, w.data_ptr(), w.stride(0),
             w_scale.data_ptr(), max(w_scale.stride(0), kb), N, out.data_ptr(), _WDTYPE[out.dtype], out.stride(0),
             1 if accumulate else 0, ptr, nbytes, _status_ptr(index))

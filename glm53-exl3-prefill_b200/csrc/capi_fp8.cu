@@ -45,12 +45,37 @@ Rows8 take_rows(Carver& c, int64_t rows, int64_t k)
     return r;
 }
 
+// Partial sums of a product whose K is split (parts > 1): fp32 [parts][rows][ld].
+struct Parts {
+    int n;
+    int64_t ld, stride;
+    float* p;
+};
+
+Parts take_parts(Carver& c, int64_t rows, int64_t E, int64_t N, int64_t K)
+{
+    Parts r{fp8_gemm_splits(rows, (int) E, (int) N, (int) K), (N + 7) / 8 * 8, 0, nullptr};
+    r.stride = rows * r.ld;
+    if (r.n > 1) r.p = c.take<float>(r.n * r.stride);
+    return r;
+}
+
+// The product of a problem that stores its sums, with K split into parts.
+int run_split(Fp8GemmProblem p, const Parts& parts, cudaStream_t stream)
+{
+    p.swiglu = 0;
+    p.out = parts.p; p.out_stride = parts.ld; p.out_dtype = EXL3_DTYPE_F32; p.accumulate = 0;
+    p.splits = parts.n; p.split_stride = parts.stride;
+    return launch_fp8_gemm(p, stream);
+}
+
 struct ExpertBuffers {
     int64_t* slot;
     void* weight_sorted;
     int32_t *expert_of_row, *counts, *row0, *meta, *scratch;
     Rows8 x, h;
-    float* y;
+    Parts gu;                       // gate | up sums, if split
+    Parts y;                        // the routes' rows: one part at least
 };
 
 ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_t d, int64_t f)
@@ -66,7 +91,9 @@ ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_
     b.scratch = c.take<int32_t>(route_sort_scratch_elems(R, (int) E));
     b.x = take_rows(c, R, d);
     b.h = take_rows(c, R, f);
-    b.y = c.take<float>(R * d);
+    b.gu = take_parts(c, R, E, 2 * f, d);
+    b.y = take_parts(c, R, E, d, f);
+    if (b.y.n == 1) b.y.p = c.take<float>(b.y.stride);
     return b;
 }
 
@@ -101,11 +128,12 @@ int check_out(const char* what, const void* out, int64_t out_dtype, int64_t T, i
     return EXL3_OK;
 }
 
-// Both products of the gated MLP over quantised rows x [rows, d]: gate | up into h, then down into `out`.
-int run_mlp(const Rows8& x, const Rows8& h, int64_t rows, int64_t d, int64_t f, int64_t E, const int32_t* counts,
-            const int32_t* row0, const void* w13, const float* w13_scale, const void* w2, const float* w2_scale,
-            double limit, void* out, int64_t out_stride, int64_t out_dtype, int accumulate, const int64_t* slot,
-            int32_t* status, cudaStream_t stream)
+// Both products of the gated MLP over quantised rows x [rows, d]: gate | up into h, then down's sums into `y` (its parts, if
+// it has several), or into `out` if y has one.
+int run_mlp(const Rows8& x, const Rows8& h, const Parts& gu, const Parts& y, int64_t rows, int64_t d, int64_t f, int64_t E,
+            const int32_t* counts, const int32_t* row0, const int32_t* rows_dev, const void* w13, const float* w13_scale,
+            const void* w2, const float* w2_scale, double limit, void* out, int64_t out_stride, int64_t out_dtype,
+            int accumulate, const int64_t* slot, int32_t* status, cudaStream_t stream)
 {
     Fp8GemmProblem p{};
     p.x = x.q; p.rows = rows; p.x_stride = d; p.K = (int) d;
@@ -116,16 +144,22 @@ int run_mlp(const Rows8& x, const Rows8& h, int64_t rows, int64_t d, int64_t f, 
     p.swiglu = 1; p.limit = (float) limit;
     p.h = h.q; p.h_stride = f; p.hs = h.s; p.hs_row = 1; p.hs_blk = rows;
     p.status = status;
-    int rc = launch_fp8_gemm(p, stream);
+    int rc = gu.n > 1 ? run_split(p, gu, stream) : launch_fp8_gemm(p, stream);
     if (rc) return rc;
+    if (gu.n > 1)
+    {
+        rc = launch_fp8_act(gu.p, gu.n, gu.stride, gu.ld, rows, rows_dev, (int) f, (float) limit, h.q, f, h.s, 1, rows, stream);
+        if (rc) return rc;
+    }
     Fp8GemmProblem q{};
     q.x = h.q; q.rows = rows; q.x_stride = f; q.K = (int) f;
     q.sx = h.s; q.sx_row = 1; q.sx_blk = rows;
     q.w = w2; q.w_stride = f; q.w_expert = d * f; q.N = (int) d; q.n_experts = (int) E;
     q.sw = w2_scale; q.sw_n = blocks128(f); q.sw_expert = blocks128(d) * q.sw_n;
     q.counts = counts; q.row0 = row0;
-    q.out = out; q.out_stride = out_stride; q.out_dtype = (int) out_dtype; q.accumulate = accumulate;
     q.slot = slot; q.status = status;
+    if (y.n > 1) return run_split(q, y, stream);
+    q.out = out; q.out_stride = out_stride; q.out_dtype = (int) out_dtype; q.accumulate = accumulate;
     return launch_fp8_gemm(q, stream);
 }
 
@@ -165,15 +199,16 @@ int exl3_fp8_quantize_rows(const void* x, int64_t dtype, int64_t rows, int64_t K
     if (rows == 0) return EXL3_OK;
     if (!x || !q || !scale) return set_error("tensors must be CUDA");
     return launch_fp8_quantize(x, (int) dtype, rows, (int) K, x_stride, pow2 ? 1 : 0, q, q_stride, scale, s_row, s_blk,
-                               nullptr, 1, nullptr, as_stream(stream));
+                               nullptr, 1, nullptr, false, as_stream(stream));
 }
 
-int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K)
+int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K, int64_t N)
 {
-    if (T < 0 || T > kMaxDim || K < 16 || K % 16 != 0 || K > (1 << 24)) return -1;
+    if (T < 0 || T > kMaxDim || K < 16 || K % 16 != 0 || K > (1 << 24) || N < 1 || N > (1 << 24)) return -1;
     if (T <= 1) return 0;                               // one row is quantised on the way
     Carver c{nullptr};
     take_rows(c, T, K);
+    if (T > kFp8FewTokens) take_parts(c, T, 1, N, K);
     return c.used;
 }
 
@@ -192,7 +227,7 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     if (!aligned16(w) || w_stride % 16 != 0 || w_stride < K)
         return set_error("fp8_linear: the weight's rows must be 16-byte aligned");
     if (w_scale_stride < blocks128(K)) return set_error("fp8_linear: weight scales [ceil(N / 128), ceil(K / 128)]");
-    if (!aligned16(workspace) || workspace_bytes < exl3_fp8_linear_workspace(T, K))
+    if (!aligned16(workspace) || workspace_bytes < exl3_fp8_linear_workspace(T, K, N))
         return set_error("fp8_linear: workspace must hold exl3_fp8_linear_workspace() bytes");
     if (T == 1)
         return launch_fp8_linear_token(x, (int) dtype, (int) K, w, w_stride, w_scale, w_scale_stride, (int) N, out,
@@ -200,7 +235,7 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     Carver c{static_cast<uint8_t*>(workspace)};
     const Rows8 r = take_rows(c, T, K);
     rc = launch_fp8_quantize(x, (int) dtype, T, (int) K, x_stride, 0, r.q, K, r.s, 1, T, nullptr, 1, nullptr,
-                             as_stream(stream));
+                             false, as_stream(stream));
     if (rc) return rc;
     Fp8GemmProblem p{};
     p.x = r.q; p.rows = T; p.x_stride = K; p.K = (int) K;
@@ -209,7 +244,12 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     p.sw = w_scale; p.sw_n = w_scale_stride; p.sw_expert = 0;
     p.out = out; p.out_stride = out_stride; p.out_dtype = (int) out_dtype; p.accumulate = accumulate ? 1 : 0;
     p.status = status;
-    return T <= kFp8FewTokens ? launch_fp8_linear_tokens(p, as_stream(stream)) : launch_fp8_gemm(p, as_stream(stream));
+    if (T <= kFp8FewTokens) return launch_fp8_linear_tokens(p, as_stream(stream));
+    const Parts parts = take_parts(c, T, 1, N, K);
+    if (parts.n == 1) return launch_fp8_gemm(p, as_stream(stream));
+    if ((rc = run_split(p, parts, as_stream(stream)))) return rc;
+    return launch_fp8_join(parts.p, parts.n, parts.stride, parts.ld, T, (int) N, accumulate ? 1 : 0, out, (int) out_dtype,
+                           out_stride, as_stream(stream));
 }
 
 int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f)
@@ -219,6 +259,8 @@ int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f)
     Carver c{nullptr};
     take_rows(c, T, d);
     take_rows(c, T, f);
+    take_parts(c, T, 1, 2 * f, d);
+    take_parts(c, T, 1, d, f);
     return c.used;
 }
 
@@ -238,11 +280,15 @@ int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_s
         return set_error("fp8_mlp: workspace must hold exl3_fp8_mlp_workspace() bytes");
     Carver c{static_cast<uint8_t*>(workspace)};
     const Rows8 xr = take_rows(c, T, d), hr = take_rows(c, T, f);
+    const Parts gu = take_parts(c, T, 1, 2 * f, d), y = take_parts(c, T, 1, d, f);
     rc = launch_fp8_quantize(x, (int) dtype, T, (int) d, x_stride, 0, xr.q, d, xr.s, 1, T, nullptr, 1, nullptr,
-                             as_stream(stream));
+                             false, as_stream(stream));
     if (rc) return rc;
-    return run_mlp(xr, hr, T, d, f, 1, nullptr, nullptr, w13, w13_scale, w2, w2_scale, limit, out, out_stride,
-                   out_dtype, accumulate ? 1 : 0, nullptr, status, as_stream(stream));
+    rc = run_mlp(xr, hr, gu, y, T, d, f, 1, nullptr, nullptr, nullptr, w13, w13_scale, w2, w2_scale, limit, out, out_stride,
+                 out_dtype, accumulate ? 1 : 0, nullptr, status, as_stream(stream));
+    if (rc || y.n == 1) return rc;
+    return launch_fp8_join(y.p, y.n, y.stride, y.ld, T, (int) d, accumulate ? 1 : 0, out, (int) out_dtype, out_stride,
+                           as_stream(stream));
 }
 
 int64_t exl3_fp8_experts_workspace(int64_t T, int64_t topk, int64_t E, int64_t d, int64_t f)
@@ -286,13 +332,13 @@ int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t
                            b.scratch, st);
     if (rc) return rc;
     rc = launch_fp8_quantize(x, (int) dtype, R, (int) d, x_stride, 0, b.x.q, d, b.x.s, 1, R, b.slot, (int) topk,
-                             b.meta + 1, st);
+                             b.meta + 1, true, st);
     if (rc) return rc;
-    rc = run_mlp(b.x, b.h, R, d, f, E, b.counts, b.row0, w13, w13_scale, w2, w2_scale, limit, b.y, d, EXL3_DTYPE_F32, 0,
-                 b.slot, status, st);
+    rc = run_mlp(b.x, b.h, b.gu, b.y, R, d, f, E, b.counts, b.row0, b.meta + 1, w13, w13_scale, w2, w2_scale, limit, b.y.p,
+                 b.y.ld, EXL3_DTYPE_F32, 0, b.slot, status, st);
     if (rc) return rc;
-    return launch_fp8_combine(b.y, d, ids, ids_is_int64 ? 1 : 0, weights, (int) weight_dtype, T, (int) topk, (int) E,
-                              (int) d, accumulate ? 1 : 0, out, (int) out_dtype, out_stride, st);
+    return launch_fp8_combine(b.y.p, b.y.ld, b.y.n, b.y.stride, ids, ids_is_int64 ? 1 : 0, weights, (int) weight_dtype, T,
+                              (int) topk, (int) E, (int) d, accumulate ? 1 : 0, out, (int) out_dtype, out_stride, st);
 }
 
 }  // extern "C"

@@ -163,10 +163,17 @@ int launch_route_logits(const void* logits, int dtype, int64_t T, int E, int64_t
 // slot (nullable): row r is x[slot[r] / topk]; rows_dev (nullable): only min(rows, *rows_dev) rows exist.
 int launch_fp8_quantize(const void* x, int dtype, int64_t rows, int K, int64_t x_stride, int pow2, void* q,
                         int64_t q_stride, float* scale, int64_t s_row, int64_t s_blk, const int64_t* slot, int topk,
-                        const int32_t* rows_dev, cudaStream_t stream);
-int launch_fp8_combine(const float* y, int64_t y_stride, const void* ids, int ids_i64, const void* weights, int wdtype,
-                       int64_t T, int topk, int E, int d, int accumulate, void* out, int out_dtype, int64_t out_stride,
-                       cudaStream_t stream);
+                        const int32_t* rows_dev, bool after, cudaStream_t stream);
+// y, part: the sum of `parts` partial sums, part_stride elements apart.  after (above; always here): launched while the
+// launch in front of it, one of these, still runs.
+int launch_fp8_combine(const float* y, int64_t y_stride, int parts, int64_t part_stride, const void* ids, int ids_i64,
+                       const void* weights, int wdtype, int64_t T, int topk, int E, int d, int accumulate, void* out,
+                       int out_dtype, int64_t out_stride, cudaStream_t stream);
+int launch_fp8_join(const float* part, int parts, int64_t part_stride, int64_t part_ld, int64_t rows, int N, int accumulate,
+                    void* out, int out_dtype, int64_t out_stride, cudaStream_t stream);
+int launch_fp8_act(const float* part, int parts, int64_t part_stride, int64_t part_ld, int64_t rows, const int32_t* rows_dev,
+                   int f, float limit, void* h, int64_t h_stride, float* hs, int64_t hs_row, int64_t hs_blk,
+                   cudaStream_t stream);
 
 // ---- fp8_gemm.cu
 struct Fp8GemmProblem {
@@ -192,8 +199,12 @@ struct Fp8GemmProblem {
     int64_t h_stride;
     float* hs;
     int64_t hs_row, hs_blk;
+    int splits;                    // > 1 (store, fp32): K in so many parts, the sums of part i at out + i * split_stride
+    int64_t split_stride;
     int32_t* status;
 };
+// Parts to split K into, for a product with few tiles.
+int fp8_gemm_splits(int64_t rows, int n_experts, int N, int K);
 int launch_fp8_gemm(const Fp8GemmProblem& p, cudaStream_t stream);
 
 // ---- fp8_small.cu

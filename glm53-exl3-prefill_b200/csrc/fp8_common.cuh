@@ -58,6 +58,31 @@ __device__ __forceinline__ float quotient(float x, float scale, float inv)
     return __uint_as_float(rest != 0.0f ? odd : u);
 }
 
+// Programmatic dependent launch.  Every kernel of the 8-bit layers lets the next launch of its stream start at once and, before
+// it touches what an earlier launch wrote (or what one may still read), waits until all of them have ended; launched
+// with launch_after() it is set up while its predecessor runs.
+__device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... Params, class... Args>
+int launch_after(const char* what, void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                 const Args&... args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (err != cudaSuccess) return set_cuda_error(what, err);
+    return check_launch(what);
+}
+
 // Two floats to e4m3 (round to nearest even), a in the low byte.
 __device__ __forceinline__ uint32_t to_e4m3x2(float a, float b)
 {

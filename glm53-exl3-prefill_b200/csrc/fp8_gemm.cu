@@ -34,7 +34,9 @@
 //   warps 2, 3    scales of the coming K blocks into a shared-memory ring (cp.async, up to eight blocks ahead);
 //   warps 4..19   four warpgroups of epilogue: warpgroup g takes 32 columns of each block (wide) or 32 tokens (thin).
 // The clusters walk the tiles (expert, weight tile, token tile; token tiles fastest, so the clusters running at
-// one time share weight tiles through L2).  Every wait is bounded as in the trellis kernels.
+// one time share weight tiles through L2).  With fewer tiles than clusters, each tile's K is split over several of them:
+// fp32 partial sums to a workspace, joined in order by the kernel that follows (fp8_rows.cu); a K block takes a cluster
+// about half a microsecond however few rows there are.  Every wait is bounded as in the trellis kernels.
 #include <cuda.h>
 
 #include "fp8_common.cuh"
@@ -62,6 +64,8 @@ struct Fp8GemmArgs {
     int N, K, n_experts;
     int n_wide, n_thin, num_kb;      // weight tiles of a wide and of a thin row tile; K blocks
     int n_blocks;                    // weight blocks of 128 rows
+    int splits;                      // clusters that share a tile's K; > 1: fp32 partial sums to out + split * split_stride
+    int64_t split_stride;
     int single_count;                // rows of the one expert when counts is null
     const int32_t* counts;           // [E] or null
     const int32_t* row0;             // [E] first row of each expert, or null
@@ -290,6 +294,7 @@ struct Tile {
     int e, nt;
     int row0, rows;                  // rows of the tile (of both CTAs)
     int ncols;                       // thin: rows rounded up to 16
+    int64_t out_offset;              // of this part of K's sums
 };
 
 // 256-row tiles of an expert with `count` rows, and whether its last rows (up to 128) are a thin tile.
@@ -335,9 +340,9 @@ constexpr int FG_STEP = 4;                                  // tokens staged at 
 
 // Eight consecutive outputs of one row.
 template <class To>
-__device__ __forceinline__ void store8(const Fp8GemmArgs& p, int64_t r, int n, const float* v)
+__device__ __forceinline__ void store8(const Fp8GemmArgs& p, const Tile& ti, int64_t r, int n, const float* v)
 {
-    To* o = reinterpret_cast<To*>(p.out) + r * p.out_stride + n;
+    To* o = reinterpret_cast<To*>(p.out) + ti.out_offset + r * p.out_stride + n;
     float a[8];
     *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(v);
     *reinterpret_cast<float4*>(a + 4) = *reinterpret_cast<const float4*>(v + 4);
@@ -365,9 +370,9 @@ __device__ __forceinline__ void write_step(const Fp8GemmArgs& p, const Tile& ti,
         if (m >= ti.rows || n >= p.N) return;
         const int64_t r = p.slot ? __ldg(p.slot + ti.row0 + m) : (int64_t) ti.row0 + m;
         const float* v = st + (tid >> 5) * 256 + c;
-        if (p.out_dtype == 0) store8<float>(p, r, n, v);
-        else if (p.out_dtype == 1) store8<__half>(p, r, n, v);
-        else store8<__nv_bfloat16>(p, r, n, v);
+        if (p.out_dtype == 0) store8<float>(p, ti, r, n, v);
+        else if (p.out_dtype == 1) store8<__half>(p, ti, r, n, v);
+        else store8<__nv_bfloat16>(p, ti, r, n, v);
     }
     else
     {
@@ -408,7 +413,7 @@ __device__ __forceinline__ void store_wide(const Fp8GemmArgs& p, const Tile& ti,
 {
     if (m >= ti.rows) return;
     const int64_t r = p.slot ? __ldg(p.slot + ti.row0 + m) : (int64_t) ti.row0 + m;
-    To* row = reinterpret_cast<To*>(p.out) + r * p.out_stride;
+    To* row = reinterpret_cast<To*>(p.out) + ti.out_offset + r * p.out_stride;
     constexpr int PER = 32 / sizeof(To);                    // values of a 32-byte sector
     #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -458,6 +463,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     __shared__ int s_pref[kMaxExperts + 1];
     __shared__ __align__(16) float s_stage[4][FG_STEP][256];
 
+    let_next_launch_start();
     const int rank = (int) cluster_rank();
     const int cluster = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -465,6 +471,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 
     if (warp == 0)
     {
+        wait_for_previous_launch();                         // (the counts are an earlier launch's)
         // tiles per expert, as an exclusive prefix
         const int per = (p.n_experts + 31) / 32;
         auto tiles = [&](int e) { return e < p.n_experts ? expert_tiles(p, e) : 0; };
@@ -512,11 +519,11 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     tc_fence_before();
     __syncthreads();
     cluster_sync();                                         // both CTAs' barriers and TMEM exist
+    wait_for_previous_launch();
     tc_fence_after();
     const uint32_t tmem_base = s_tmem_base;
     volatile int* abort_flag = &s_abort;
-    const int total = s_pref[p.n_experts];
-    const int nkb = p.num_kb;
+    const int total = s_pref[p.n_experts] * p.splits;       // work units: (tile, part of K), parts fastest
 
     if (warp < 4)
     {
@@ -529,7 +536,8 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             bool ok = true;
             for (int t = cluster; ok && t < total; t += n_clusters)
             {
-                const Tile ti = tile_at(p, s_pref, t);
+                const Tile ti = tile_at(p, s_pref, t / p.splits);
+                const int split = t % p.splits, kb0 = split * p.num_kb / p.splits, kb1 = (split + 1) * p.num_kb / p.splits;
                 // rows of this CTA's first and last box, boxes, and the pair's bytes: wide, one weight block and up to
                 // 128 tokens a CTA; thin, two weight blocks and half of the columns of each half
                 const int nc1 = max(ti.ncols - 64, 0), nc0 = ti.ncols - nc1;
@@ -542,7 +550,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 const int w_row0 = weight_block<SWIGLU>(p, ti, rank, ti.thin ? 0 : rank) * kBlock;
                 const int w_row1 = weight_block<SWIGLU>(p, ti, rank, 1) * kBlock;
                 const uint32_t x_off = ti.thin ? 2 * FG_W_BYTES : FG_W_BYTES;
-                for (int kb = 0; kb < nkb; ++kb, ++issued, st.next())
+                for (int kb = kb0; kb < kb1; ++kb, ++issued, st.next())
                 {
                     // (the first pass does not wait: a fresh barrier counts as past the phase of parity 1)
                     ok = warp_wait(&bar_done[st.slot], st.parity ^ 1u, abort_flag, p.status, p.wait_ns);
@@ -576,9 +584,10 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 bool ok = true;
                 for (int t = cluster; ok && t < total; t += n_clusters)
                 {
-                    const Tile ti = tile_at(p, s_pref, t);
+                    const Tile ti = tile_at(p, s_pref, t / p.splits);
+                    const int split = t % p.splits, kb0 = split * p.num_kb / p.splits, kb1 = (split + 1) * p.num_kb / p.splits;
                     const int nc1 = max(ti.ncols - 64, 0), nc0 = ti.ncols - nc1;
-                    for (int kb = 0; kb < nkb; ++kb, st.next(), buf.next())
+                    for (int kb = kb0; kb < kb1; ++kb, st.next(), buf.next())
                     {
                         // one round trip to shared memory for the three barriers of a K block: this warp's own
                         // instructions are what the loop waits for once the sums keep up
@@ -638,12 +647,14 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             bool ok = true;
             for (int t = cluster; ok && t < total; t += n_clusters)
             {
-                const Tile ti = tile_at(p, s_pref, t);
+                const Tile ti = tile_at(p, s_pref, t / p.splits);
+                const int split = t % p.splits, kb0 = split * p.num_kb / p.splits, kb1 = (split + 1) * p.num_kb / p.splits;
                 const int rows = ti.thin ? ti.rows : min(128, ti.rows - 128 * rank);
-                const float* sx = p.sx + (int64_t) (ti.row0 + (ti.thin ? 0 : 128 * rank) + j) * p.sx_row;
+                const float* sx = p.sx + (int64_t) (ti.row0 + (ti.thin ? 0 : 128 * rank) + j) * p.sx_row + kb0 * p.sx_blk;
                 // a block past the last one has sums of zero: any scale will do
-                const float* sw = p.sw + ti.e * p.sw_expert + min(weight_block<SWIGLU>(p, ti, rank, j & 1), p.n_blocks - 1) * p.sw_n;
-                for (int kb = 0; kb < nkb; ++kb, sr.next())
+                const float* sw = p.sw + ti.e * p.sw_expert + min(weight_block<SWIGLU>(p, ti, rank, j & 1), p.n_blocks - 1) * p.sw_n +
+                                  kb0;
+                for (int kb = kb0; kb < kb1; ++kb, sr.next())
                 {
                     const int q = sr.slot;
                     ok = warp_wait(&bar_sempty[q], sr.parity ^ 1u, abort_flag, p.status, p.wait_ns);
@@ -673,7 +684,9 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         uint64_t* bar_sums = g >> 1 ? bar_done : bar_half;
         for (int t = cluster; t < total; t += n_clusters)
         {
-            Tile ti = tile_at(p, s_pref, t);
+            Tile ti = tile_at(p, s_pref, t / p.splits);
+            const int split = t % p.splits, kb0 = split * p.num_kb / p.splits, kb1 = (split + 1) * p.num_kb / p.splits;
+            ti.out_offset = split * p.split_stride;
             uint64_t acc[2][16];                            // 32 columns (wide) or tokens (thin) of each block
             #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -682,7 +695,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             const bool work = !ti.thin || g * 32 < ti.rows;
             bool ok = true;
             #pragma unroll 1
-            for (int kb = 0; kb < nkb; ++kb)
+            for (int kb = kb0; kb < kb1; ++kb)
             {
                 const int q = sr.slot;
                 if (!__all_sync(0xffffffffu, mbar_test_wait2(&bar_sfull[q], sr.parity, &bar_sums[sg.slot], sg.parity)))
@@ -917,13 +930,28 @@ int launch_fp8_gemm(const Fp8GemmProblem& q, cudaStream_t stream)
         return 0;
     });
     if (rc) return rc;
+    p.splits = q.splits > 1 ? q.splits : 1;
+    p.split_stride = q.split_stride;
     // tiles are counted on the device; this bound only keeps the grid from being larger than the work
-    const int64_t tiles = (q.rows / 256 + (q.rows < q.n_experts ? q.rows : q.n_experts)) * p.n_wide;
+    const int64_t tiles = (q.rows / 256 + (q.rows < q.n_experts ? q.rows : q.n_experts)) * p.n_wide * p.splits;
     const int64_t most = max_clusters();
-    const unsigned grid = 2u * (unsigned) (tiles < most ? tiles : most);
-    if (q.swiglu) fp8_gemm_kernel<true><<<grid, FG_THREADS, kDynBytes, stream>>>(tw, tx, p);
-    else fp8_gemm_kernel<false><<<grid, FG_THREADS, kDynBytes, stream>>>(tw, tx, p);
-    return check_launch("fp8_gemm");
+    const dim3 grid(2u * (unsigned) (tiles < most ? tiles : most));
+    return q.swiglu ? launch_after("fp8_gemm", fp8_gemm_kernel<true>, grid, FG_THREADS, kDynBytes, stream, tw, tx, p)
+                    : launch_after("fp8_gemm", fp8_gemm_kernel<false>, grid, FG_THREADS, kDynBytes, stream, tw, tx, p);
+}
+
+int fp8_gemm_splits(int64_t rows, int n_experts, int N, int K)
+{
+    // the clusters of a B200 (148 SMs, some without a partner), the tiles there will be (an expert's last rows taken for
+    // a thin tile), and at least four K blocks a part
+    constexpr int64_t clusters = 72;
+    const int64_t units = (N + 255) / 256, kb = (K + FG_BK - 1) / FG_BK;
+    const int64_t experts = rows < n_experts ? rows : n_experts;
+    const int64_t tiles = rows / 256 * units + experts * ((units + 1) / 2);
+    int64_t s = clusters / (tiles > 0 ? tiles : 1);
+    if (s > kb / 4) s = kb / 4;
+    if (s > 8) s = 8;
+    return s < 2 ? 1 : (int) s;
 }
 
 }  // namespace exl3b

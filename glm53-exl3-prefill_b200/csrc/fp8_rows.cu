@@ -49,7 +49,8 @@ template <class T, int ALIGN, bool POW2, class Index>
 __global__ __launch_bounds__(Q_THREADS)
 void quantize_rows_kernel(const QuantArgs p)
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // a product that follows may fetch its weights
+    let_next_launch_start();
+    wait_for_previous_launch();
     const int lane8 = threadIdx.x & 7;
     const int64_t rows = p.rows_dev ? min(p.rows, (int64_t) *p.rows_dev) : p.rows;
     const Index units = (Index) (rows * p.n_blocks);                // (row, block) pairs, blocks fastest
@@ -115,6 +116,8 @@ void quantize_rows_kernel(const QuantArgs p)
 struct CombineArgs {
     const float* y;
     int64_t y_stride;
+    int parts;                       // y is the sum of this many, part_stride elements apart
+    int64_t part_stride;
     const void* ids;
     int ids_i64;
     const void* weights;
@@ -124,6 +127,18 @@ struct CombineArgs {
     void* out;
     int64_t out_stride;
 };
+
+// Four values as the sum of `parts` partial sums, in order.
+__device__ __forceinline__ float4 sum_parts(const float* y, int parts, int64_t stride)
+{
+    float4 v = *reinterpret_cast<const float4*>(y);
+    for (int i = 1; i < parts; ++i)
+    {
+        const float4 o = *reinterpret_cast<const float4*>(y + i * stride);
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+    }
+    return v;
+}
 
 __device__ __forceinline__ float route_weight(const void* w, int dtype, int64_t i)
 {
@@ -136,6 +151,8 @@ template <class To>
 __global__ __launch_bounds__(256)
 void combine_routes_kernel(const CombineArgs p)
 {
+    let_next_launch_start();
+    wait_for_previous_launch();
     const int64_t t = blockIdx.y + (int64_t) blockIdx.z * 65535;
     if (t >= p.T) return;
     const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -152,7 +169,7 @@ void combine_routes_kernel(const CombineArgs p)
                                     : (int64_t) __ldg(reinterpret_cast<const int*>(p.ids) + s);
         if (e < 0 || e >= p.E) continue;
         const float w = route_weight(p.weights, p.wdtype, s);
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p.y + s * p.y_stride + c));
+        const float4 v = sum_parts(p.y + s * p.y_stride + c, p.parts, p.part_stride);
         a[0] = fmaf(w, v.x, a[0]);
         a[1] = fmaf(w, v.y, a[1]);
         a[2] = fmaf(w, v.z, a[2]);
@@ -162,27 +179,101 @@ void combine_routes_kernel(const CombineArgs p)
     for (int i = 0; i < 4; ++i) out[i] = from_float<To>(a[i]);
 }
 
-template <class T, int ALIGN>
-void launch_quant(const QuantArgs& p, bool pow2, unsigned grid, cudaStream_t stream)
+// ------------------------------------------------------------------------------------ products split along K
+// out[r, n] = (accumulate ? out[r, n] : 0) + the parts' sum; N is the valid width, parts hold rows of part_ld values.
+struct JoinArgs {
+    const float* part;
+    int parts;
+    int64_t part_stride, part_ld;
+    int64_t rows;
+    int N, accumulate;
+    void* out;
+    int64_t out_stride;
+};
+
+template <class To>
+__global__ __launch_bounds__(256)
+void join_parts_kernel(const JoinArgs p)
 {
+    let_next_launch_start();
+    wait_for_previous_launch();
+    const int per_row = (p.N + 3) / 4;
+    for (int64_t u = (int64_t) blockIdx.x * 256 + threadIdx.x; u < p.rows * per_row; u += (int64_t) gridDim.x * 256)
+    {
+        const int64_t r = u / per_row;
+        const int n = (int) (u - r * per_row) * 4;
+        const float4 v = sum_parts(p.part + r * p.part_ld + n, p.parts, p.part_stride);
+        const float a[4] = {v.x, v.y, v.z, v.w};
+        To* o = reinterpret_cast<To*>(p.out) + r * p.out_stride + n;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < p.N) o[i] = from_float<To>(p.accumulate ? to_float(o[i]) + a[i] : a[i]);
+    }
+}
+
+// The gate and up halves of a row (columns 0..f-1 and f..2f-1 of the parts) to quantised activations: a warp per row and block of
+// 128 columns, 4 a lane.
+struct ActArgs {
+    const float* part;
+    int parts;
+    int64_t part_stride, part_ld;
+    int64_t rows;
+    const int32_t* rows_dev;
+    int f;
+    float limit;
+    uint8_t* h;
+    int64_t h_stride;
+    float* hs;
+    int64_t hs_row, hs_blk;
+};
+
+__global__ __launch_bounds__(256)
+void act_parts_kernel(const ActArgs p)
+{
+    let_next_launch_start();
+    wait_for_previous_launch();
+    const int lane = threadIdx.x & 31, blocks = p.f / kBlock;
+    const int64_t rows = p.rows_dev ? min(p.rows, (int64_t) *p.rows_dev) : p.rows;
+    for (int64_t u = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5); u < rows * blocks; u += (int64_t) gridDim.x * 8)
+    {
+        const int64_t r = u / blocks;
+        const int b = (int) (u - r * blocks);
+        const float* y = p.part + r * p.part_ld + b * kBlock + 4 * lane;
+        const float4 g = sum_parts(y, p.parts, p.part_stride), w = sum_parts(y + p.f, p.parts, p.part_stride);
+        const float a[4] = {clamped_swiglu(g.x, w.x, p.limit), clamped_swiglu(g.y, w.y, p.limit),
+                            clamped_swiglu(g.z, w.z, p.limit), clamped_swiglu(g.w, w.w, p.limit)};
+        uint32_t m = 0;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(a[i]) & 0x7fffffffu);
+        const float s = block_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, m)), false), inv = reciprocal(s);
+        float q[4];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = quotient(a[i], s, inv);
+        reinterpret_cast<uint32_t*>(p.h + r * p.h_stride + b * kBlock)[lane] =
+            to_e4m3x2(q[0], q[1]) | to_e4m3x2(q[2], q[3]) << 16;
+        if (lane == 0) p.hs[r * p.hs_row + b * p.hs_blk] = s;
+    }
+}
+
+template <class T, int ALIGN>
+int launch_quant(const QuantArgs& p, bool pow2, unsigned grid, bool after, cudaStream_t stream)
+{
+    auto go = [&](void (*kernel)(QuantArgs)) {
+        if (after) return launch_after("fp8_quantize_rows", kernel, dim3(grid), Q_THREADS, 0, stream, p);
+        kernel<<<grid, Q_THREADS, 0, stream>>>(p);
+        return check_launch("fp8_quantize_rows");
+    };
     const bool small = p.rows * p.n_blocks < (1LL << 31);           // (row, block) numbers fit 32 bits: cheap divisions
     if (pow2)
-    {
-        if (small) quantize_rows_kernel<T, ALIGN, true, uint32_t><<<grid, Q_THREADS, 0, stream>>>(p);
-        else quantize_rows_kernel<T, ALIGN, true, uint64_t><<<grid, Q_THREADS, 0, stream>>>(p);
-    }
-    else
-    {
-        if (small) quantize_rows_kernel<T, ALIGN, false, uint32_t><<<grid, Q_THREADS, 0, stream>>>(p);
-        else quantize_rows_kernel<T, ALIGN, false, uint64_t><<<grid, Q_THREADS, 0, stream>>>(p);
-    }
+        return go(small ? quantize_rows_kernel<T, ALIGN, true, uint32_t> : quantize_rows_kernel<T, ALIGN, true, uint64_t>);
+    return go(small ? quantize_rows_kernel<T, ALIGN, false, uint32_t> : quantize_rows_kernel<T, ALIGN, false, uint64_t>);
 }
 
 }  // namespace
 
 int launch_fp8_quantize(const void* x, int dtype, int64_t rows, int K, int64_t x_stride, int pow2, void* q,
                         int64_t q_stride, float* scale, int64_t s_row, int64_t s_blk, const int64_t* slot, int topk,
-                        const int32_t* rows_dev, cudaStream_t stream)
+                        const int32_t* rows_dev, bool after, cudaStream_t stream)
 {
     QuantArgs p{};
     p.x = x; p.x_stride = x_stride; p.K = K; p.n_blocks = (K + kBlock - 1) / kBlock;
@@ -197,26 +288,48 @@ int launch_fp8_quantize(const void* x, int dtype, int64_t rows, int K, int64_t x
     const unsigned grid = (unsigned) (ctas < most ? ctas : most);
     auto go = [&](auto v) {
         using T = decltype(v);
-        if (align == 32) launch_quant<T, 32>(p, pow2 != 0, grid, stream);
-        else if (align == 16) launch_quant<T, 16>(p, pow2 != 0, grid, stream);
-        else launch_quant<T, 0>(p, pow2 != 0, grid, stream);
+        if (align == 32) return launch_quant<T, 32>(p, pow2 != 0, grid, after, stream);
+        if (align == 16) return launch_quant<T, 16>(p, pow2 != 0, grid, after, stream);
+        return launch_quant<T, 0>(p, pow2 != 0, grid, after, stream);
     };
-    if (dtype == 0) go(float{});
-    else if (dtype == 1) go(__half{});
-    else go(__nv_bfloat16{});
-    return check_launch("fp8_quantize_rows");
+    if (dtype == 0) return go(float{});
+    if (dtype == 1) return go(__half{});
+    return go(__nv_bfloat16{});
 }
 
-int launch_fp8_combine(const float* y, int64_t y_stride, const void* ids, int ids_i64, const void* weights, int wdtype,
-                       int64_t T, int topk, int E, int d, int accumulate, void* out, int out_dtype, int64_t out_stride,
-                       cudaStream_t stream)
+int launch_fp8_combine(const float* y, int64_t y_stride, int parts, int64_t part_stride, const void* ids, int ids_i64,
+                       const void* weights, int wdtype, int64_t T, int topk, int E, int d, int accumulate, void* out,
+                       int out_dtype, int64_t out_stride, cudaStream_t stream)
 {
-    CombineArgs p{y, y_stride, ids, ids_i64, weights, wdtype, T, topk, E, d, accumulate, out, out_stride};
+    const CombineArgs p{y, y_stride, parts, part_stride, ids, ids_i64, weights, wdtype, T, topk, E, d, accumulate, out,
+                        out_stride};
     const dim3 grid((unsigned) ((d / 4 + 255) / 256), (unsigned) (T < 65535 ? T : 65535), (unsigned) ((T + 65534) / 65535));
-    if (out_dtype == 0) combine_routes_kernel<float><<<grid, 256, 0, stream>>>(p);
-    else if (out_dtype == 1) combine_routes_kernel<__half><<<grid, 256, 0, stream>>>(p);
-    else combine_routes_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
-    return check_launch("fp8_combine");
+    const char* what = "fp8_combine";
+    if (out_dtype == 0) return launch_after(what, combine_routes_kernel<float>, grid, 256, 0, stream, p);
+    if (out_dtype == 1) return launch_after(what, combine_routes_kernel<__half>, grid, 256, 0, stream, p);
+    return launch_after(what, combine_routes_kernel<__nv_bfloat16>, grid, 256, 0, stream, p);
+}
+
+int launch_fp8_join(const float* part, int parts, int64_t part_stride, int64_t part_ld, int64_t rows, int N, int accumulate,
+                    void* out, int out_dtype, int64_t out_stride, cudaStream_t stream)
+{
+    const JoinArgs p{part, parts, part_stride, part_ld, rows, N, accumulate, out, out_stride};
+    const int64_t ctas = (rows * ((N + 3) / 4) + 255) / 256, most = (int64_t) device_sm_count() * 8;
+    const dim3 grid((unsigned) (ctas < most ? ctas : most));
+    const char* what = "fp8_join";
+    if (out_dtype == 0) return launch_after(what, join_parts_kernel<float>, grid, 256, 0, stream, p);
+    if (out_dtype == 1) return launch_after(what, join_parts_kernel<__half>, grid, 256, 0, stream, p);
+    return launch_after(what, join_parts_kernel<__nv_bfloat16>, grid, 256, 0, stream, p);
+}
+
+int launch_fp8_act(const float* part, int parts, int64_t part_stride, int64_t part_ld, int64_t rows, const int32_t* rows_dev,
+                   int f, float limit, void* h, int64_t h_stride, float* hs, int64_t hs_row, int64_t hs_blk,
+                   cudaStream_t stream)
+{
+    const ActArgs p{part, parts, part_stride, part_ld, rows, rows_dev, f, limit, static_cast<uint8_t*>(h), h_stride, hs,
+                    hs_row, hs_blk};
+    const int64_t ctas = (rows * (f / kBlock) + 7) / 8, most = (int64_t) device_sm_count() * 8;
+    return launch_after("fp8_act", act_parts_kernel, dim3((unsigned) (ctas < most ? ctas : most)), 256, 0, stream, p);
 }
 
 }  // namespace exl3b

@@ -61,10 +61,6 @@ __device__ __forceinline__ void load_frag(const uint8_t* row, int kb, int t, int
     }
 }
 
-// Programmatic dependent launch: let the next launch of the stream start; wait for the previous one's results.
-__device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // Four consecutive values of a block (columns 4 lane .. 4 lane + 3 of block kb), zeros past K.  `vec`: 4-value loads.
 template <class T>
 __device__ __forceinline__ void load_values(const T* x, int kb, int lane, int K, bool vec, float (&v)[4])
@@ -215,6 +211,7 @@ __global__ __launch_bounds__(T_THREADS, 2)
 void linear_token_kernel(const SmallLinearArgs p)
 {
     __shared__ float s_sum[T_WARPS][16];
+    let_next_launch_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * 16, g = lane >> 2;
     const int nkb = (p.K + kBlock - 1) / kBlock;
@@ -247,6 +244,7 @@ void linear_tokens_kernel(const SmallLinearArgs p)
 {
     constexpr int DEPTH = NG;                              // blocks of weights in flight per warp
     __shared__ float s_sum[WARPS][16][NG * 8];
+    let_next_launch_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n0 = blockIdx.x * 16, g = lane >> 2, t = lane & 3;
     const int nkb = (p.K + kBlock - 1) / kBlock;
@@ -427,24 +425,6 @@ void down_token_kernel(const SmallExpertArgs p)
     }
 }
 
-// A launch that may start before the one in front of it on the stream has ended (its kernel waits for that itself).
-template <class Args>
-int launch_dependent(void (*kernel)(Args), dim3 grid, int threads, cudaStream_t stream, const Args& args, const char* what)
-{
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, args);
-    if (err != cudaSuccess) return set_cuda_error(what, err);
-    return check_launch(what);
-}
-
 }  // namespace
 
 int launch_fp8_linear_token(const void* x, int dtype, int K, const void* w, int64_t w_stride, const float* sw, int64_t sw_n,
@@ -481,10 +461,10 @@ int launch_fp8_linear_tokens(const Fp8GemmProblem& q, cudaStream_t stream)
     // two groups of columns need twice the registers, so half the warps with twice the blocks in flight
     const char* what = "fp8_linear (few tokens)";
     if (q.rows <= 8)
-        return a32 ? launch_dependent(linear_tokens_kernel<1, T_WARPS, true>, dim3(grid), T_THREADS, stream, p, what)
-                   : launch_dependent(linear_tokens_kernel<1, T_WARPS, false>, dim3(grid), T_THREADS, stream, p, what);
-    return a32 ? launch_dependent(linear_tokens_kernel<2, S_WARPS, true>, dim3(grid), S_THREADS, stream, p, what)
-               : launch_dependent(linear_tokens_kernel<2, S_WARPS, false>, dim3(grid), S_THREADS, stream, p, what);
+        return a32 ? launch_after(what, linear_tokens_kernel<1, T_WARPS, true>, dim3(grid), T_THREADS, 0, stream, p)
+                   : launch_after(what, linear_tokens_kernel<1, T_WARPS, false>, dim3(grid), T_THREADS, 0, stream, p);
+    return a32 ? launch_after(what, linear_tokens_kernel<2, S_WARPS, true>, dim3(grid), S_THREADS, 0, stream, p)
+               : launch_after(what, linear_tokens_kernel<2, S_WARPS, false>, dim3(grid), S_THREADS, 0, stream, p);
 }
 
 int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_stride, const void* ids, int ids_i64,
@@ -506,8 +486,8 @@ int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_s
     else gate_up_token_kernel<__nv_bfloat16><<<grid, S_THREADS, 0, stream>>>(p);
     int rc = check_launch("fp8_experts (gate and up, few routes)");
     if (rc) return rc;
-    return launch_dependent(down_token_kernel, dim3((unsigned) (d / 16), (unsigned) T), T_THREADS, stream, p,
-                            "fp8_experts (down, few routes)");
+    return launch_after("fp8_experts (down, few routes)", down_token_kernel, dim3((unsigned) (d / 16), (unsigned) T),
+                        T_THREADS, 0, stream, p);
 }
 
 }  // namespace exl3b

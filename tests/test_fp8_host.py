@@ -59,8 +59,8 @@ def test_quantize_refusals(lib):
 
 
 def test_linear_refusals(lib):
-    need = lib.exl3_fp8_linear_workspace(4, 256)
-    assert need >= 4 * 256 + 4 * 2 * 4 and lib.exl3_fp8_linear_workspace(4, 100) == -1
+    need = lib.exl3_fp8_linear_workspace(4, 256, 64)
+    assert need >= 4 * 256 + 4 * 2 * 4 and lib.exl3_fp8_linear_workspace(4, 100, 64) == -1
 
     def call(T=4, K=256, xs=256, w=A, wstride=256, wss=2, N=64, out=A, odt=0, ostride=64, ws=A, nbytes=need):
         return lib.exl3_fp8_linear(A, 1, T, K, xs, w, wstride, A, wss, N, out, odt, ostride, 0, ws, nbytes, None, None)

@@ -213,14 +213,15 @@ def test_linear_no_rows(ext, cuda_device):
 
 
 # ------------------------------------------------------------------------------------ gated MLP and experts
-@pytest.mark.parametrize("T", [1, 7, 32, 33, 128, 200])
-def test_mlp(ext, cuda_device, T):
+@pytest.mark.parametrize("T,d,f", [(1, 384, 256), (7, 384, 256), (32, 384, 256), (33, 384, 256), (128, 384, 256),
+                                   (200, 384, 256), (40, 1024, 1024), (130, 1152, 640), (300, 2048, 512)])
+def test_mlp(ext, cuda_device, T, d, f):
     dev = cuda_device
-    L = make_layer(1, 384, 256, 11, dev)
-    x = rows(T, 384, torch.bfloat16, dev, T)
+    L = make_layer(1, d, f, 11, dev)
+    x = rows(T, d, torch.bfloat16, dev, T)
     want = ref_mlp(x, L, 0)
     assert rel(exl3_fp8.fp8_mlp_prefill(x, L, LIMIT), want) <= MLP_REL
-    base = torch.randn(T, 384, device=dev)
+    base = torch.randn(T, d, device=dev)
     out = exl3_dense.dense_mlp_prefill(x, L, LIMIT, out=base.clone())
     assert rel(out - base, want) <= MLP_REL + 1e-5
     assert ext.read_status(dev) == 0
@@ -229,7 +230,7 @@ def test_mlp(ext, cuda_device, T):
 @pytest.mark.parametrize("T,E,d,f,k,kind", [
     (1, 1, 128, 128, 1, "uniform"), (1, 288, 512, 256, 8, "uniform"), (3, 8, 256, 384, 8, "uniform"),
     (40, 16, 256, 128, 2, "zipf"), (256, 16, 1024, 512, 4, "uniform"), (300, 5, 384, 256, 3, "zipf"),
-    (1000, 8, 256, 256, 2, "skewed"), (5, 1024, 128, 128, 4, "uniform")])
+    (20, 4, 1024, 512, 2, "uniform"), (90, 3, 1280, 1152, 2, "zipf"), (1000, 8, 256, 256, 2, "skewed"), (5, 1024, 128, 128, 4, "uniform")])
 def test_experts(ext, cuda_device, T, E, d, f, k, kind):
     dev = cuda_device
     L = make_layer(E, d, f, 21, dev)
