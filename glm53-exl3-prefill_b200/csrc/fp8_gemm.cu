@@ -186,8 +186,8 @@ __device__ __forceinline__ void cp_async_wait_all()
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Non-blocking test of one phase each of two barriers.
-__device__ __forceinline__ bool mbar_test_wait2(uint64_t* bar_a, uint32_t parity_a, uint64_t* bar_b, uint32_t parity_b)
+// Non-blocking test of one phase each of two barriers (shared-memory addresses).
+__device__ __forceinline__ bool mbar_test2(uint32_t bar_a, uint32_t parity_a, uint32_t bar_b, uint32_t parity_b)
 {
     uint32_t done;
     asm volatile(
@@ -196,7 +196,7 @@ __device__ __forceinline__ bool mbar_test_wait2(uint64_t* bar_a, uint32_t parity
         "mbarrier.test_wait.parity.shared::cta.b64 pb, [%3], %4;\n\t"
         "and.pred pa, pa, pb;\n\t"
         "selp.u32 %0, 1, 0, pa;\n\t}"
-        : "=r"(done) : "r"(smem_u32(bar_a)), "r"(parity_a), "r"(smem_u32(bar_b)), "r"(parity_b) : "memory");
+        : "=r"(done) : "r"(bar_a), "r"(parity_a), "r"(bar_b), "r"(parity_b) : "memory");
     return done != 0;
 }
 
@@ -677,16 +677,21 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         const int g = (warp - 4) >> 2;                      // warpgroup
         const int quarter = warp & 3;
         const int lane_in = quarter * 32 + lane;            // TMEM lane: token (wide) or weight row (thin)
+        // registers are short here (64 of sums, 16 on their way): positions from one counter, 32-bit addresses
         Ring<FG_STAGES> sg;
-        Ring<FG_SCALES> sr;
-        int b = 0;                                          // TMEM buffer
+        uint32_t it = 0;
         const uint32_t tempty = in_cta0(&bar_tempty[2 * (g >> 1)]);
-        uint64_t* bar_sums = g >> 1 ? bar_done : bar_half;
+        const uint32_t sums = smem_u32(g >> 1 ? bar_done : bar_half);
+        const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (g >> 1) * 256 + (g & 1) * 32;
         for (int t = cluster; t < total; t += n_clusters)
         {
             Tile ti = tile_at(p, s_pref, t / p.splits);
-            const int split = t % p.splits, kb0 = split * p.num_kb / p.splits, kb1 = (split + 1) * p.num_kb / p.splits;
-            ti.out_offset = split * p.split_stride;
+            int blocks;                                     // K blocks of this part
+            {
+                const int split = t % p.splits;
+                ti.out_offset = split * p.split_stride;
+                blocks = (split + 1) * p.num_kb / p.splits - split * p.num_kb / p.splits;
+            }
             uint64_t acc[2][16];                            // 32 columns (wide) or tokens (thin) of each block
             #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -695,18 +700,17 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             const bool work = !ti.thin || g * 32 < ti.rows;
             bool ok = true;
             #pragma unroll 1
-            for (int kb = kb0; kb < kb1; ++kb)
+            for (; blocks > 0; --blocks)
             {
-                const int q = sr.slot;
-                if (!__all_sync(0xffffffffu, mbar_test_wait2(&bar_sfull[q], sr.parity, &bar_sums[sg.slot], sg.parity)))
+                const uint32_t q = it % FG_SCALES, q_parity = (it / FG_SCALES) & 1u;
+                if (!__all_sync(0xffffffffu, mbar_test2(smem_u32(bar_sfull) + q * 8, q_parity, sums + sg.slot * 8, sg.parity)))
                 {
-                    ok = warp_wait(&bar_sfull[q], sr.parity, abort_flag, p.status, p.wait_ns) &&
-                         warp_wait(&bar_sums[sg.slot], sg.parity, abort_flag, p.status, p.wait_ns);
+                    ok = warp_wait(&bar_sfull[q], q_parity, abort_flag, p.status, p.wait_ns) &&
+                         warp_wait(&(g >> 1 ? bar_done : bar_half)[sg.slot], sg.parity, abort_flag, p.status, p.wait_ns);
                     if (!ok) break;
                 }
                 tc_fence_after();
-                const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (2 * (g >> 1) + b) * 128 +
-                                       (g & 1) * 32;
+                const uint32_t taddr = tmem + (it & 1u) * 128;
                 if (!ti.thin)
                 {
                     const float x = s_sx[q][lane_in];
@@ -753,12 +757,11 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 __syncwarp();
                 if (lane == 0)
                 {
-                    mbar_arrive_cluster(tempty + b * 8);
+                    mbar_arrive_cluster(tempty + (it & 1u) * 8);
                     mbar_arrive(&bar_sempty[q]);
                 }
-                b ^= 1;
+                ++it;
                 sg.next();
-                sr.next();
             }
             // A warp that gave up says so before the epilogue's barrier, and every warp reads it between this
             // barrier and the next: one decision for all of them.
