@@ -69,10 +69,15 @@ int run_split(Fp8GemmProblem p, const Parts& parts, cudaStream_t stream)
     return launch_fp8_gemm(p, stream);
 }
 
+// Whether rows are quantised once per token and copied to their routes (two launches), or once per route (one).  At 4096
+// columns and 8 routes a token, per route and per token: 8192 tokens 190 and 95 us, 2048 55 and 30, 512 16 and 14.
+bool many_routes(int64_t R, int64_t topk) { return topk > 1 && R >= 4096; }
+
 struct ExpertBuffers {
     int64_t* slot;
     void* weight_sorted;
     int32_t *expert_of_row, *counts, *row0, *meta, *scratch;
+    Rows8 tokens;                   // quantised once per token, if that pays
     Rows8 x, h;
     Parts gu;                       // gate | up sums, if split
     Parts y;                        // the routes' rows: one part at least
@@ -89,6 +94,7 @@ ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_
     b.row0 = c.take<int32_t>(E);
     b.meta = c.take<int32_t>(2);
     b.scratch = c.take<int32_t>(route_sort_scratch_elems(R, (int) E));
+    if (many_routes(R, topk)) b.tokens = take_rows(c, T, d);
     b.x = take_rows(c, R, d);
     b.h = take_rows(c, R, f);
     b.gu = take_parts(c, R, E, 2 * f, d);
@@ -98,8 +104,9 @@ ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_
 }
 
 // Routes whose products each read their expert's weights for themselves (fp8_small.cu), activations [R, f] in the workspace.
-constexpr int64_t kFewRoutes = 32;
-bool few_routes(int64_t R) { return R <= kFewRoutes; }
+// With 288 experts of 4096 x 1536 (every route another expert), 8 / 16 / 32 / 64 routes: 40 / 71 / 125 / 257 us, and 58 / 95 /
+// 138 / 203 us by the tiles of fp8_gemm.cu; where routes share experts the tiles read the weights once, hence the second bound.
+bool few_routes(int64_t R, int64_t E) { return R <= 32 && R <= 2 * E; }
 
 int check_rows(const char* what, int64_t dtype, int64_t rows, int64_t K, int64_t stride)
 {
@@ -257,8 +264,12 @@ int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f)
     if (T < 0 || T > kMaxDim || d <= 0 || d % 128 != 0 || d > (1 << 24) || f <= 0 || f % 128 != 0 || f > (1 << 24))
         return -1;
     Carver c{nullptr};
+    if (few_routes(T, 1)) c.take<float>(T * f);
+    if (few_routes(T, 1)) return c.used;
     take_rows(c, T, d);
     take_rows(c, T, f);
+    if (T <= kFp8FewTokens) c.take<float>(T * 2 * f);
+    if (T <= kFp8FewTokens) return c.used;
     take_parts(c, T, 1, 2 * f, d);
     take_parts(c, T, 1, d, f);
     return c.used;
@@ -279,7 +290,30 @@ int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_s
     if (!aligned16(workspace) || workspace_bytes < exl3_fp8_mlp_workspace(T, d, f))
         return set_error("fp8_mlp: workspace must hold exl3_fp8_mlp_workspace() bytes");
     Carver c{static_cast<uint8_t*>(workspace)};
+    if (few_routes(T, 1))
+        return launch_fp8_experts_small(x, (int) dtype, (int) T, (int) d, x_stride, nullptr, 0, nullptr, 0, 1, 1, w13,
+                                        w13_scale, w2, w2_scale, (int) f, (float) limit, c.take<float>(T * f), out,
+                                        (int) out_dtype, out_stride, accumulate ? 1 : 0, as_stream(stream));
     const Rows8 xr = take_rows(c, T, d), hr = take_rows(c, T, f);
+    if (T <= kFp8FewTokens)
+    {
+        // the same four steps by the kernels for few tokens: rows, gate | up sums, activations, down
+        float* sums = c.take<float>(T * 2 * f);
+        rc = launch_fp8_quantize(x, (int) dtype, T, (int) d, x_stride, 0, xr.q, d, xr.s, 1, T, nullptr, 1, nullptr, false,
+                                 as_stream(stream));
+        if (rc) return rc;
+        Fp8GemmProblem p{};
+        p.x = xr.q; p.rows = T; p.x_stride = d; p.K = (int) d; p.sx = xr.s; p.sx_row = 1; p.sx_blk = T;
+        p.w = w13; p.w_stride = d; p.N = (int) (2 * f); p.sw = w13_scale; p.sw_n = blocks128(d);
+        p.out = sums; p.out_stride = 2 * f; p.out_dtype = EXL3_DTYPE_F32;
+        if ((rc = launch_fp8_linear_tokens(p, as_stream(stream)))) return rc;
+        rc = launch_fp8_act(sums, 1, 0, 2 * f, T, nullptr, (int) f, (float) limit, hr.q, f, hr.s, 1, T, as_stream(stream));
+        if (rc) return rc;
+        p.x = hr.q; p.x_stride = f; p.K = (int) f; p.sx = hr.s;
+        p.w = w2; p.w_stride = f; p.N = (int) d; p.sw = w2_scale; p.sw_n = blocks128(f);
+        p.out = out; p.out_stride = out_stride; p.out_dtype = (int) out_dtype; p.accumulate = accumulate ? 1 : 0;
+        return launch_fp8_linear_tokens(p, as_stream(stream));
+    }
     const Parts gu = take_parts(c, T, 1, 2 * f, d), y = take_parts(c, T, 1, d, f);
     rc = launch_fp8_quantize(x, (int) dtype, T, (int) d, x_stride, 0, xr.q, d, xr.s, 1, T, nullptr, 1, nullptr,
                              false, as_stream(stream));
@@ -294,7 +328,7 @@ int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_s
 int64_t exl3_fp8_experts_workspace(int64_t T, int64_t topk, int64_t E, int64_t d, int64_t f)
 {
     if (check_experts_shape("fp8_experts", T, topk, E, d, f)) return -1;
-    if (few_routes(T * topk)) return up256(T * topk * f * (int64_t) sizeof(float));
+    if (few_routes(T * topk, E)) return up256(T * topk * f * (int64_t) sizeof(float));
     Carver c{nullptr};
     take_experts(c, T, topk, E, d, f);
     return c.used;
@@ -319,7 +353,7 @@ int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t
         return set_error("fp8_experts: workspace must hold exl3_fp8_experts_workspace() bytes");
     cudaStream_t st = as_stream(stream);
     const int64_t R = T * topk;
-    if (few_routes(R))
+    if (few_routes(R, E))
         return launch_fp8_experts_small(x, (int) dtype, (int) T, (int) d, x_stride, ids, ids_is_int64 ? 1 : 0, weights,
                                         (int) weight_dtype, (int) topk, (int) E, w13, w13_scale, w2, w2_scale, (int) f,
                                         (float) limit, static_cast<float*>(workspace), out, (int) out_dtype, out_stride,
@@ -331,8 +365,16 @@ int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t
                            b.weight_sorted, b.expert_of_row, b.counts, b.row0, nullptr, nullptr, b.meta, nullptr,
                            b.scratch, st);
     if (rc) return rc;
-    rc = launch_fp8_quantize(x, (int) dtype, R, (int) d, x_stride, 0, b.x.q, d, b.x.s, 1, R, b.slot, (int) topk,
-                             b.meta + 1, true, st);
+    if (many_routes(R, topk))
+    {
+        rc = launch_fp8_quantize(x, (int) dtype, T, (int) d, x_stride, 0, b.tokens.q, d, b.tokens.s, 1, T, nullptr, 1,
+                                 nullptr, true, st);
+        if (rc) return rc;
+        rc = launch_fp8_gather(b.tokens.q, b.tokens.s, T, b.slot, (int) topk, (int) d, b.meta + 1, b.x.q, b.x.s, R, st);
+    }
+    else
+        rc = launch_fp8_quantize(x, (int) dtype, R, (int) d, x_stride, 0, b.x.q, d, b.x.s, 1, R, b.slot, (int) topk,
+                                 b.meta + 1, true, st);
     if (rc) return rc;
     rc = run_mlp(b.x, b.h, b.gu, b.y, R, d, f, E, b.counts, b.row0, b.meta + 1, w13, w13_scale, w2, w2_scale, limit, b.y.p,
                  b.y.ld, EXL3_DTYPE_F32, 0, b.slot, status, st);

@@ -164,6 +164,9 @@ int launch_route_logits(const void* logits, int dtype, int64_t T, int E, int64_t
 int launch_fp8_quantize(const void* x, int dtype, int64_t rows, int K, int64_t x_stride, int pow2, void* q,
                         int64_t q_stride, float* scale, int64_t s_row, int64_t s_blk, const int64_t* slot, int topk,
                         const int32_t* rows_dev, bool after, cudaStream_t stream);
+// Quantised rows [tokens, d] (scales [d / 128][tokens]) copied to the rows of their routes ([rows, d], [d / 128][rows]).
+int launch_fp8_gather(const void* q, const float* s, int64_t tokens, const int64_t* slot, int topk, int d,
+                      const int32_t* rows_dev, void* q_out, float* s_out, int64_t rows, cudaStream_t stream);
 // y, part: the sum of `parts` partial sums, part_stride elements apart.  after (above; always here): launched while the
 // launch in front of it, one of these, still runs.
 int launch_fp8_combine(const float* y, int64_t y_stride, int parts, int64_t part_stride, const void* ids, int ids_i64,
@@ -212,6 +215,7 @@ constexpr int kFp8FewTokens = 16;      // most rows of launch_fp8_linear_tokens
 int launch_fp8_linear_token(const void* x, int dtype, int K, const void* w, int64_t w_stride, const float* sw, int64_t sw_n,
                             int N, void* out, int out_dtype, int accumulate, cudaStream_t stream);
 int launch_fp8_linear_tokens(const Fp8GemmProblem& p, cudaStream_t stream);
+// ids, weights null: a plain MLP (topk 1, one expert, weight 1).
 int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_stride, const void* ids, int ids_i64,
                              const void* weights, int wdtype, int topk, int E, const void* w13, const float* s13,
                              const void* w2, const float* s2, int f, float limit, float* act, void* out, int out_dtype,

@@ -110,6 +110,47 @@ void quantize_rows_kernel(const QuantArgs p)
     }
 }
 
+// ------------------------------------------------------------------------------------ rows by route
+// Quantised rows of tokens copied to their routes' places: row r of q, s is token slot[r] / topk's.  With many routes per
+// token this is cheaper than quantising every route's copy (65536 routes of 4096 columns from 8192 tokens: 206 us).
+struct GatherArgs {
+    const uint8_t* q;
+    const float* s;                  // [blocks][tokens]
+    int64_t tokens;
+    const int64_t* slot;
+    int topk, d;
+    const int32_t* rows_dev;
+    uint8_t* q_out;
+    float* s_out;                    // [blocks][rows]
+    int64_t rows;
+};
+
+__global__ __launch_bounds__(256)
+void gather_rows_kernel(const GatherArgs p)
+{
+    let_next_launch_start();
+    wait_for_previous_launch();
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = min(p.rows, (int64_t) *p.rows_dev), n = p.d / 16;
+    for (int64_t r = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t) gridDim.x * 8)
+    {
+        const int64_t t = (int64_t) ((uint32_t) p.slot[r] / (uint32_t) p.topk);
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + t * p.d);
+        uint4* dst = reinterpret_cast<uint4*>(p.q_out + r * p.d);
+        for (int64_t i = lane; i < n; i += 128)
+        {
+            uint4 v[4];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + 32 * j < n) v[j] = src[i + 32 * j];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + 32 * j < n) dst[i + 32 * j] = v[j];
+        }
+        for (int b = lane; b < p.d / kBlock; b += 32) p.s_out[b * p.rows + r] = p.s[b * p.tokens + t];
+    }
+}
+
 // ------------------------------------------------------------------------------------ sum over a token's routes
 //     out[t] = (accumulate ? out[t] : 0) + sum over j ascending, ids[t, j] in [0, E), of w[t, j] * y[t * topk + j]
 // in fp32 and a fixed order (no atomics), rounded once to out's type.  Bound by reading y.
@@ -295,6 +336,15 @@ int launch_fp8_quantize(const void* x, int dtype, int64_t rows, int K, int64_t x
     if (dtype == 0) return go(float{});
     if (dtype == 1) return go(__half{});
     return go(__nv_bfloat16{});
+}
+
+int launch_fp8_gather(const void* q, const float* s, int64_t tokens, const int64_t* slot, int topk, int d,
+                      const int32_t* rows_dev, void* q_out, float* s_out, int64_t rows, cudaStream_t stream)
+{
+    const GatherArgs p{static_cast<const uint8_t*>(q), s, tokens, slot, topk, d, rows_dev, static_cast<uint8_t*>(q_out),
+                       s_out, rows};
+    const int64_t ctas = (rows + 7) / 8, most = (int64_t) device_sm_count() * 16;
+    return launch_after("fp8_gather", gather_rows_kernel, dim3((unsigned) (ctas < most ? ctas : most)), 256, 0, stream, p);
 }
 
 int launch_fp8_combine(const float* y, int64_t y_stride, int parts, int64_t part_stride, const void* ids, int ids_i64,

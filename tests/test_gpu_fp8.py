@@ -213,7 +213,8 @@ def test_linear_no_rows(ext, cuda_device):
 
 
 # ------------------------------------------------------------------------------------ gated MLP and experts
-@pytest.mark.parametrize("T,d,f", [(1, 384, 256), (7, 384, 256), (32, 384, 256), (33, 384, 256), (128, 384, 256),
+@pytest.mark.parametrize("T,d,f", [(1, 384, 256), (2, 640, 384), (3, 384, 256), (7, 384, 256),
+                                   (8, 1280, 384), (16, 384, 256), (17, 384, 256), (32, 384, 256), (33, 384, 256), (128, 384, 256),
                                    (200, 384, 256), (40, 1024, 1024), (130, 1152, 640), (300, 2048, 512)])
 def test_mlp(ext, cuda_device, T, d, f):
     dev = cuda_device
@@ -230,6 +231,7 @@ def test_mlp(ext, cuda_device, T, d, f):
 @pytest.mark.parametrize("T,E,d,f,k,kind", [
     (1, 1, 128, 128, 1, "uniform"), (1, 288, 512, 256, 8, "uniform"), (3, 8, 256, 384, 8, "uniform"),
     (40, 16, 256, 128, 2, "zipf"), (256, 16, 1024, 512, 4, "uniform"), (300, 5, 384, 256, 3, "zipf"),
+    (4, 4, 512, 256, 2, "uniform"), (16, 16, 512, 256, 2, "zipf"), (2100, 8, 256, 128, 2, "zipf"),
     (20, 4, 1024, 512, 2, "uniform"), (90, 3, 1280, 1152, 2, "zipf"), (1000, 8, 256, 256, 2, "skewed"), (5, 1024, 128, 128, 4, "uniform")])
 def test_experts(ext, cuda_device, T, E, d, f, k, kind):
     dev = cuda_device
