@@ -11,12 +11,16 @@ allocations take longer than the kernels (one token: 0.24 ms per layer through t
 ``max_tokens``) into a CUDA graph with static input and output buffers and replays it: a call copies
 its inputs into the bucket's buffers (padding tokens get expert id -1, which the sort leaves unrouted),
 replays the graph and returns a view of the bucket's fp32 output.  Results equal ``grouped_prefill``'s
-(bit for bit with deterministic=True; with the atomic down stage up to the order of the fp32 adds).
+(bit for bit with deterministic=True; with the atomic down stage up to the order of the fp32 adds).  A layer of
+8-bit experts (exl3_fp8) is replayed alike; its inputs are held in fp32, so that any input type keeps its
+values, and results are those of grouped_prefill on the padded bucket (fp32 rounding apart from the same call
+without padding, which other kernels may take).
 """
 from __future__ import annotations
 
 import torch
 
+import exl3_fp8
 import exl3_grouped_runtime as rt
 
 
@@ -29,8 +33,10 @@ class GraphedPrefill:
             raise RuntimeError("max_tokens must be positive")
         self.layer, self.limit, self.topk = layer, float(limit), int(topk)
         self.deterministic = rt.deterministic_default() if deterministic is None else bool(deterministic)
-        self.device = device if device is not None else layer.w13_trellis.device
-        self.d = int(layer.w13_trellis.shape[2]) * 16
+        self.fp8 = exl3_fp8.is_fp8_layer(layer)
+        weights = layer.w13_fp8 if self.fp8 else layer.w13_trellis
+        self.device = device if device is not None else weights.device
+        self.d = int(weights.shape[2]) * (1 if self.fp8 else 16)
         self.max_tokens = int(max_tokens)
         self._graphs = {}                  # bucket -> (graph, x, ids, w, out)
 
@@ -43,7 +49,7 @@ class GraphedPrefill:
 
     def _capture(self, b: int):
         dev = self.device
-        x = torch.zeros(b, self.d, dtype=torch.float16, device=dev)
+        x = torch.zeros(b, self.d, dtype=torch.float32 if self.fp8 else torch.float16, device=dev)
         ids = torch.full((b, self.topk), -1, dtype=torch.int64, device=dev)
         w = torch.zeros(b, self.topk, dtype=torch.float32, device=dev)
         # warm up on a side stream: loads the library and sets every kernel attribute before the capture

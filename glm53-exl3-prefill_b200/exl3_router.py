@@ -16,6 +16,7 @@ from __future__ import annotations
 import torch
 
 import b200_ext
+import exl3_fp8
 import exl3_grouped_runtime as rt
 
 
@@ -82,7 +83,14 @@ def moe_prefill_from_hidden(x2d: torch.Tensor, router: NoauxTcRouter, layer, lim
                             stage_hook=None, return_routing: bool = False, deterministic: bool | None = None):
     """Hidden states [T, d] -> routed-expert output fp32 [T, d] (+ the shared expert if given), with the
     router and the sort on the GPU.  With return_routing, also returns (ids, weights).  `deterministic`
-    as for grouped_prefill."""
+    as for grouped_prefill.  8-bit experts (exl3_fp8) take the router's ids and weights as they are."""
+    if exl3_fp8.is_fp8_layer(layer):
+        import exl3_dense
+        if int(layer.w13_fp8.shape[0]) != router.n_experts:
+            raise RuntimeError("the router and the layer disagree on the number of experts")
+        ids, w = router.route(x2d)
+        out = exl3_dense.moe_block_prefill(x2d, ids, w, layer, shared, limit, stage_hook=stage_hook)
+        return (out, ids, w) if return_routing else out
     if deterministic is None:
         deterministic = rt.deterministic_default()
     hook = stage_hook if stage_hook is not None else (lambda name: None)

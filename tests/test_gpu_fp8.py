@@ -290,6 +290,24 @@ def test_block_from_logits_with_8_bit_layers(ext, cuda_device):
     assert names[-2:] == ["shared_fp8_mlp", "end"]
 
 
+def test_graphed_small_batches_and_the_hidden_state_router(ext, cuda_device):
+    import exl3_decode
+    dev = cuda_device
+    E, d, f, k = 16, 256, 128, 4
+    L, S = make_layer(E, d, f, 61, dev), make_layer(1, d, f, 63, dev)
+    graphed = exl3_decode.GraphedPrefill(L, LIMIT, k, max_tokens=16)
+    for T in (1, 3, 16):
+        ids, w = (t.to(dev) for t in synth.routing("uniform", T, E, k, seed=T))
+        x = rows(T, d, torch.bfloat16, dev, T)
+        assert rel(graphed(x, ids, w), ref_experts(x, ids, w, L)) <= MLP_REL
+    g = torch.Generator(device=dev).manual_seed(7)
+    router = exl3_router.NoauxTcRouter(torch.randn(E, d, generator=g, device=dev) / d ** 0.5, topk=k)
+    x = rows(50, d, torch.float16, dev, 9)
+    out, ids, w = exl3_router.moe_prefill_from_hidden(x, router, L, LIMIT, shared=S, return_routing=True)
+    assert rel(out, ref_experts(x, ids, w, L) + ref_mlp(x, S, 0)) <= MLP_REL
+    assert ext.read_status(dev) == 0
+
+
 def test_two_graphs_on_two_streams(ext, cuda_device):
     """Two captured calls share nothing: replayed side by side they give the eager results."""
     dev = cuda_device

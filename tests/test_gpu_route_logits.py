@@ -15,6 +15,7 @@ pytestmark = pytest.mark.gpu
 W_REL = 2.0 ** -17
 
 
+@np.errstate(over="ignore", invalid="ignore")
 def reference(logits, bias, k, softmax, n_group, topk_group, group_top, norm, scale):
     """The definition, one token at a time, in Python floats (64 bits)."""
     l = logits.double().cpu().numpy()
