@@ -294,6 +294,7 @@ struct Tile {
     int e, nt;
     int row0, rows;                  // rows of the tile (of both CTAs)
     int ncols;                       // thin: rows rounded up to 16
+    int kb0, kb1;                    // its K blocks
     int64_t out_offset;              // of this part of K's sums
 };
 
@@ -312,14 +313,26 @@ __device__ __forceinline__ int expert_tiles(const Fp8GemmArgs& p, int e)
     return wide_tiles(count) * p.n_wide + thin_tiles(count) * p.n_thin;
 }
 
+// Work unit t: a tile, or a part of its K.
 __device__ __forceinline__ Tile tile_at(const Fp8GemmArgs& p, const int* pref, int t)
 {
     Tile ti;
-    ti.e = trellis::prefix_find(pref, p.n_experts, t);
+    ti.kb0 = 0;
+    ti.kb1 = p.num_kb;
+    ti.out_offset = 0;
+    if (p.splits > 1)                                       // (divisions only where they are needed)
+    {
+        const int tile = t / p.splits, split = t - tile * p.splits;
+        ti.kb0 = split * p.num_kb / p.splits;
+        ti.kb1 = (split + 1) * p.num_kb / p.splits;
+        ti.out_offset = split * p.split_stride;
+        t = tile;
+    }
+    ti.e = p.n_experts > 1 ? trellis::prefix_find(pref, p.n_experts, t) : 0;
     const int count = row_count(p, ti.e), wide = wide_tiles(count);
-    const int local = t - pref[ti.e];
+    const int local = p.n_experts > 1 ? t - pref[ti.e] : t;
     ti.thin = local >= wide * p.n_wide;
-    ti.nt = ti.thin ? local - wide * p.n_wide : local / wide;
+    ti.nt = ti.thin ? local - wide * p.n_wide : wide > 1 ? local / wide : local;
     const int first = ti.thin ? count / 256 * 256 : (local - ti.nt * wide) * 256;
     ti.row0 = (p.row0 ? __ldg(p.row0 + ti.e) : 0) + first;
     ti.rows = min(256, count - first);
@@ -536,8 +549,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             bool ok = true;
             for (int t = cluster; ok && t < total; t += n_clusters)
             {
-                const Tile ti = tile_at(p, s_pref, t / p.splits);
-                const int split = t % p.splits, kb0 = split * p.num_kb / p.splits, kb1 = (split + 1) * p.num_kb / p.splits;
+                const Tile ti = tile_at(p, s_pref, t);
                 // rows of this CTA's first and last box, boxes, and the pair's bytes: wide, one weight block and up to
                 // 128 tokens a CTA; thin, two weight blocks and half of the columns of each half
                 const int nc1 = max(ti.ncols - 64, 0), nc0 = ti.ncols - nc1;
@@ -550,7 +562,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 const int w_row0 = weight_block<SWIGLU>(p, ti, rank, ti.thin ? 0 : rank) * kBlock;
                 const int w_row1 = weight_block<SWIGLU>(p, ti, rank, 1) * kBlock;
                 const uint32_t x_off = ti.thin ? 2 * FG_W_BYTES : FG_W_BYTES;
-                for (int kb = kb0; kb < kb1; ++kb, ++issued, st.next())
+                for (int kb = ti.kb0; kb < ti.kb1; ++kb, ++issued, st.next())
                 {
                     // (the first pass does not wait: a fresh barrier counts as past the phase of parity 1)
                     ok = warp_wait(&bar_done[st.slot], st.parity ^ 1u, abort_flag, p.status, p.wait_ns);
@@ -584,10 +596,9 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 bool ok = true;
                 for (int t = cluster; ok && t < total; t += n_clusters)
                 {
-                    const Tile ti = tile_at(p, s_pref, t / p.splits);
-                    const int split = t % p.splits, kb0 = split * p.num_kb / p.splits, kb1 = (split + 1) * p.num_kb / p.splits;
+                    const Tile ti = tile_at(p, s_pref, t);
                     const int nc1 = max(ti.ncols - 64, 0), nc0 = ti.ncols - nc1;
-                    for (int kb = kb0; kb < kb1; ++kb, st.next(), buf.next())
+                    for (int kb = ti.kb0; kb < ti.kb1; ++kb, st.next(), buf.next())
                     {
                         // one round trip to shared memory for the three barriers of a K block: this warp's own
                         // instructions are what the loop waits for once the sums keep up
@@ -647,14 +658,13 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             bool ok = true;
             for (int t = cluster; ok && t < total; t += n_clusters)
             {
-                const Tile ti = tile_at(p, s_pref, t / p.splits);
-                const int split = t % p.splits, kb0 = split * p.num_kb / p.splits, kb1 = (split + 1) * p.num_kb / p.splits;
+                const Tile ti = tile_at(p, s_pref, t);
                 const int rows = ti.thin ? ti.rows : min(128, ti.rows - 128 * rank);
-                const float* sx = p.sx + (int64_t) (ti.row0 + (ti.thin ? 0 : 128 * rank) + j) * p.sx_row + kb0 * p.sx_blk;
+                const float* sx = p.sx + (int64_t) (ti.row0 + (ti.thin ? 0 : 128 * rank) + j) * p.sx_row + ti.kb0 * p.sx_blk;
                 // a block past the last one has sums of zero: any scale will do
                 const float* sw = p.sw + ti.e * p.sw_expert + min(weight_block<SWIGLU>(p, ti, rank, j & 1), p.n_blocks - 1) * p.sw_n +
-                                  kb0;
-                for (int kb = kb0; kb < kb1; ++kb, sr.next())
+                                  ti.kb0;
+                for (int kb = ti.kb0; kb < ti.kb1; ++kb, sr.next())
                 {
                     const int q = sr.slot;
                     ok = warp_wait(&bar_sempty[q], sr.parity ^ 1u, abort_flag, p.status, p.wait_ns);
@@ -685,13 +695,8 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (g >> 1) * 256 + (g & 1) * 32;
         for (int t = cluster; t < total; t += n_clusters)
         {
-            Tile ti = tile_at(p, s_pref, t / p.splits);
-            int blocks;                                     // K blocks of this part
-            {
-                const int split = t % p.splits;
-                ti.out_offset = split * p.split_stride;
-                blocks = (split + 1) * p.num_kb / p.splits - split * p.num_kb / p.splits;
-            }
+            Tile ti = tile_at(p, s_pref, t);
+            int blocks = ti.kb1 - ti.kb0;
             uint64_t acc[2][16];                            // 32 columns (wide) or tokens (thin) of each block
             #pragma unroll
             for (int h = 0; h < 2; ++h)
