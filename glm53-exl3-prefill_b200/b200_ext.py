@@ -479,8 +479,9 @@ def fp8_linear(x, w, w_scale, out, accumulate=False):
     if w.dtype != _E4M3 or w.dim() != 2 or w.shape[1] != K or (K > 1 and w.stride(1) != 1):
         _fail("fp8_linear: weight e4m3 [N, K] with contiguous rows")
     N, kb = w.shape[0], -(-K // 128)
-    if w_scale.dtype != torch.float32 or w_scale.shape != (-(-N // 128), kb) or (kb > 1 and w_scale.stride(1) != 1):
-        _fail("fp8_linear: weight_scale fp32 [ceil(N/128), ceil(K/128)]")
+    if (w_scale.dtype != torch.float32 or w_scale.shape != (-(-N // 128), kb) or (kb > 1 and w_scale.stride(1) != 1)
+            or (N > 128 and w_scale.stride(0) < kb)):
+        _fail("fp8_linear: weight_scale fp32 [ceil(N/128), ceil(K/128)] with contiguous, separate rows")
     index = _gpu_of(x, w, w_scale, out)
     _check_out(out, T, N, "fp8_linear")
     if K % 16:

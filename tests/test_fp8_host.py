@@ -140,6 +140,15 @@ def test_python_refusals(lib):
         exl3_fp8.fp8_prefill(x, ids, rw, L, 7.0)
 
 
+def test_broadcast_weight_scales_are_refused(lib):
+    """Scales with a row stride of 0 would be read past their end: refused before a launch."""
+    x = torch.zeros(4, 256)
+    w = torch.zeros(300, 256, dtype=torch.float8_e4m3fn)
+    for scale in (torch.ones(1, 2).expand(3, 2), torch.ones(1).expand(3, 2), torch.ones(2, 3).t()):
+        with pytest.raises(RuntimeError, match="weight_scale"):
+            exl3_fp8.fp8_linear(x, w, scale)
+
+
 @pytest.mark.parametrize("shape", [(128, 128), (1, 16), (200, 300), (3, 130, 256)])
 def test_quantize_weight(shape):
     w = torch.randn(*shape, generator=torch.Generator().manual_seed(1))
