@@ -487,9 +487,9 @@ def fp8_linear(x, w, w_scale, out, accumulate=False):
     if K % 16:
         _fail("fp8_linear: K must be a multiple of 16")
     ws, ptr, nbytes = _workspace(index, "exl3_fp8_linear_workspace", T, K, N)
-    _launch(index, load().exl3_fp8_linear, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, w.data_ptr(), w.stride(0),
-            w_scale.data_ptr(), max(w_scale.stride(0), kb), N, out.data_ptr(), _WDTYPE[out.dtype], out.stride(0),
-            1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
+    _launch(index, load().exl3_fp8_linear, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, w.data_ptr(),
+            w.stride(0) if N > 1 else K, w_scale.data_ptr(), max(w_scale.stride(0), kb), N, out.data_ptr(),
+            _WDTYPE[out.dtype], out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
 
 
 def _check_fp8_layer(w13, s13, w2, s2, d, what):

@@ -16,6 +16,12 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 int64_t up256(int64_t n) { return (n + 255) & ~int64_t(255); }
 int64_t blocks128(int64_t n) { return (n + 127) / 128; }
 bool is_dtype(int64_t d) { return d >= EXL3_DTYPE_F32 && d <= EXL3_DTYPE_BF16; }
+int64_t bytes_of(int64_t dtype) { return dtype == EXL3_DTYPE_F32 ? 4 : 2; }
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t) b_bytes && y < x + (uintptr_t) a_bytes;
+}
 
 constexpr int64_t kMaxDim = 0x7fffff00;
 
@@ -211,7 +217,11 @@ int exl3_fp8_quantize_rows(const void* x, int64_t dtype, int64_t rows, int64_t K
 
 int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K, int64_t N)
 {
-    if (T < 0 || T > kMaxDim || K < 16 || K % 16 != 0 || K > (1 << 24) || N < 1 || N > (1 << 24)) return -1;
+    if (T < 0 || T > kMaxDim || K < 16 || K % 16 != 0 || K > (1 << 24) || N < 1 || N > (1 << 24))
+    {
+        set_error("fp8_linear: invalid sizes (K must be a multiple of 16, K and N 1..2^24)");
+        return -1;
+    }
     if (T <= 1) return 0;                               // one row is quantised on the way
     Carver c{nullptr};
     take_rows(c, T, K);
@@ -236,6 +246,8 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     if (w_scale_stride < blocks128(K)) return set_error("fp8_linear: weight scales [ceil(N / 128), ceil(K / 128)]");
     if (!aligned16(workspace) || workspace_bytes < exl3_fp8_linear_workspace(T, K, N))
         return set_error("fp8_linear: workspace must hold exl3_fp8_linear_workspace() bytes");
+    if (T == 1 && overlap(x, K * bytes_of(dtype), out, N * bytes_of(out_dtype)))
+        return set_error("fp8_linear: out overlaps x (one token is read while out is written)");
     if (T == 1)
         return launch_fp8_linear_token(x, (int) dtype, (int) K, w, w_stride, w_scale, w_scale_stride, (int) N, out,
                                        (int) out_dtype, accumulate ? 1 : 0, as_stream(stream));
@@ -261,8 +273,7 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
 
 int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f)
 {
-    if (T < 0 || T > kMaxDim || d <= 0 || d % 128 != 0 || d > (1 << 24) || f <= 0 || f % 128 != 0 || f > (1 << 24))
-        return -1;
+    if (check_experts_shape("fp8_mlp", T, 1, 1, d, f)) return -1;
     Carver c{nullptr};
     if (few_routes(T, 1)) c.take<float>(T * f);
     if (few_routes(T, 1)) return c.used;

@@ -62,7 +62,8 @@ def quantize_weight(w: torch.Tensor):
 def fp8_linear(x2d: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
                out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """x2d [T, K], weight e4m3 [N, K], weight_scale fp32 [ceil(N/128), ceil(K/128)] -> x W^T [T, N] as out_dtype
-    (float32, float16 or bfloat16), or added into `out` if given.  K must be a multiple of 16."""
+    (float32, float16 or bfloat16), or added into `out` if given.  K must be a multiple of 16; with one token `out`
+    may not overlap x (refused)."""
     if x2d.dim() != 2 or weight.dim() != 2 or x2d.size(1) != weight.size(1):
         raise RuntimeError("fp8_linear: K mismatch between x [T, K] and weight [N, K]")
     accumulate = out is not None

@@ -256,7 +256,8 @@ EXL3_API int exl3_fp8_quantize_rows(const void* x, int64_t dtype, int64_t rows, 
                                     int64_t s_blk, void* stream);
 
 /* out [T, N] = quantised(x) . W^T (added to out if accumulate).  W e4m3 [N, K] (row stride w_stride, 16-byte
- * aligned rows), w_scale [ceil(N / 128), ceil(K / 128)] with row stride w_scale_stride.  K % 16 == 0. */
+ * aligned rows), w_scale [ceil(N / 128), ceil(K / 128)] with row stride w_scale_stride.  K % 16 == 0.  With one
+ * token out must not overlap x (refused). */
 EXL3_API int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K, int64_t N);      /* bytes; -1: bad arguments */
 EXL3_API int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t x_stride, const void* w,
                              int64_t w_stride, const float* w_scale, int64_t w_scale_stride, int64_t N, void* out,

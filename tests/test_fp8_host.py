@@ -149,6 +149,20 @@ def test_broadcast_weight_scales_are_refused(lib):
             exl3_fp8.fp8_linear(x, w, scale)
 
 
+def test_one_token_linear_refuses_an_output_that_overlaps_its_input(lib):
+    def call(T, x, out, ws=None, nbytes=0):
+        return lib.exl3_fp8_linear(P(x), 1, T, 256, 256, A, 256, A, 2, 64, P(out), 0, 64, 1, ws, nbytes, None, None)
+    for x, out in [(4096, 4096), (4096, 4096 + 511), (4096 + 255, 4096), (4096, 4096 - 255)]:
+        refused(lib, call(1, x, out), "overlaps x")
+
+
+def test_workspace_sizes_name_their_refusal(lib):
+    assert lib.exl3_fp8_linear_workspace(4, 0, 64) == -1
+    assert "fp8_linear: invalid sizes" in lib.exl3_last_error().decode()
+    assert lib.exl3_fp8_mlp_workspace(4, 256, 64) == -1
+    assert "f must be a multiple of 128" in lib.exl3_last_error().decode()
+
+
 @pytest.mark.parametrize("shape", [(128, 128), (1, 16), (200, 300), (3, 130, 256)])
 def test_quantize_weight(shape):
     w = torch.randn(*shape, generator=torch.Generator().manual_seed(1))
