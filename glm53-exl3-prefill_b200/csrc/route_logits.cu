@@ -7,7 +7,9 @@
 //     ids  = the topk experts by c among the topk_group groups with the largest G, best first
 //     w    = s[ids] / (sum s[ids] + 1e-20) (the division only if norm) * scale
 // Ties go to the lower expert (group) number.  Logits that are NaN or -inf are masked: never chosen, and
-// outside the softmax; a token with fewer than topk experts left gets id -1 and weight 0 in its last slots.
+// outside the softmax; a bias of NaN or -inf only keeps its expert from being chosen, and
+// +inf counts as the largest float.  A token with fewer than topk
+// experts left gets id -1 and weight 0 in its last slots.
 // The sigmoid router of GLM-5.3-Flash (docs/research/02-glm-5.3-flash-architecture.md:33) is the case
 // of one group; router.cu fuses that case with the router's product for callers that hold hidden states.
 //
@@ -107,16 +109,17 @@ __device__ __forceinline__ float fast_sigmoid(float l)
     return r;
 }
 
+// A bias of +inf as the largest float, so that sums with masked experts stay out of NaN.
+__device__ __forceinline__ float bounded(float b) { return b > 3.402823466e38f ? 3.402823466e38f : b; }
+
 // The selection score of expert e in 64 bits (inv: the softmax's 1 / sum, in 64 bits).
 template <bool SOFTMAX>
 __device__ __forceinline__ double exact_score(const RouteLogitsArgs& p, float l, int e, float m, double inv)
 {
     const double s = SOFTMAX ? (l == m ? 1.0 : exp((double) l - (double) m)) * inv : 1.0 / (1.0 + exp(-(double) l));
-    return p.bias ? s + (double) p.bias[e] : s;
+    return p.bias ? s + (double) bounded(p.bias[e]) : s;
 }
 
-// The token's whole selection in 64 bits, by one warp: lane j < topk returns the expert of slot j (-1: none).  A path for
-// more than 32 candidates that nearly tie, written for its size: scores are computed again wherever needed.
 // 1 / sum of the softmax in 64 bits.
 template <class Tl>
 __device__ __forceinline__ double exact_inverse_sum(const RouteLogitsArgs& p, const Tl* row, float m, int lane)
@@ -153,14 +156,21 @@ __device__ __noinline__ int rank_in_64_bits(const RouteLogitsArgs& p, const Tl* 
     return out;
 }
 
+template <class F> __device__ __forceinline__ F lowest();
+template <> __device__ __forceinline__ float lowest() { return -INFINITY; }
+template <> __device__ __forceinline__ double lowest() { return -(double) INFINITY; }
+
+// The token's whole selection in 64 bits, by one warp: lane j < topk returns the expert of slot j (-1: none).  A path for
+// more than 32 candidates that nearly tie, written for its size: scores are computed again wherever needed.
 template <bool SOFTMAX, class Tl>
 __device__ __noinline__ int select_in_64_bits(const RouteLogitsArgs& p, const Tl* row, float m, int lane, unsigned kept)
 {
     const double inv = SOFTMAX ? exact_inverse_sum(p, row, m, lane) : 1.0;
     auto score = [&](int e, bool& ok) {
         const float l = load_logit(row + e);
-        ok = l > -INFINITY;
-        return exact_score<SOFTMAX>(p, l, e, m, inv);
+        const double c = exact_score<SOFTMAX>(p, l, e, m, inv);
+        ok = l > -INFINITY && c > lowest<double>();
+        return c;
     };
     // the best expert in [lo, hi) that comes after (pv, pe) in the order: larger score first, then lower number
     auto next = [&](int lo, int hi, unsigned groups, double pv, int pe, double& bv) {
@@ -194,10 +204,6 @@ __device__ __noinline__ int select_in_64_bits(const RouteLogitsArgs& p, const Tl
     }
     return mine;
 }
-
-template <class F> __device__ __forceinline__ F lowest();
-template <> __device__ __forceinline__ float lowest() { return -INFINITY; }
-template <> __device__ __forceinline__ double lowest() { return -(double) INFINITY; }
 
 // The groups kept (a bit each) by their scores, from the token's selection scores sc[E] in shared memory; `gap`: how far
 // the last kept group's score is above the best dropped one's, and `low` the former.  lanes_per_group lanes scan a group and
@@ -245,7 +251,8 @@ __device__ __noinline__ unsigned kept_groups_in_64_bits(const RouteLogitsArgs& p
     for (int e = lane; e < p.E; e += 32)
     {
         const float l = load_logit(row + e);
-        sc[e] = l > -INFINITY ? exact_score<SOFTMAX>(p, l, e, m, inv) : lowest<double>();
+        const double c = exact_score<SOFTMAX>(p, l, e, m, inv);
+        sc[e] = l > -INFINITY && c > lowest<double>() ? c : lowest<double>();
     }
     __syncwarp();
     double low, gap;
@@ -270,7 +277,7 @@ void route_logits_kernel(const __grid_constant__ RouteLogitsArgs p)
     for (int i = 0; i < MPL; ++i)
     {
         const int e = lane + 32 * i;
-        bias[i] = by_score && e < p.E ? __ldg(p.bias + e) : 0.0f;
+        bias[i] = by_score && e < p.E ? bounded(__ldg(p.bias + e)) : 0.0f;
         group[i] = e < p.E ? 1u << (e / p.per_group) : 0u;
     }
     for (int64_t t = (int64_t) blockIdx.x * RL_WARPS + warp; t < p.T; t += (int64_t) gridDim.x * RL_WARPS)
@@ -303,7 +310,7 @@ void route_logits_kernel(const __grid_constant__ RouteLogitsArgs p)
         {
             float c = v[i];
             if (by_score) c = (SOFTMAX ? fast_exp(c, m) * inv : fast_sigmoid(c)) + bias[i];
-            key[i] = v[i] == v[i] ? order_key(c) : 0u;
+            key[i] = c > -INFINITY ? order_key(c) : 0u;                     // masked by its logit (NaN here) or its bias
         }
         unsigned kept = ~0u;
         if (grouped)

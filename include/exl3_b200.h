@@ -234,8 +234,9 @@ EXL3_API int exl3_fat_gemm_scatter(const void* a, int64_t size_m, int64_t size_k
  *   ids = the topk experts by c inside the topk_group groups with the largest scores, best first;
  *   weights = s[ids] / (sum + 1e-20) if norm else s[ids], times scale.
  * Ties go to the lower expert (group), and the choice is that of exact arithmetic.  NaN and -inf logits are
- * masked (never chosen); missing experts give id -1 and weight 0.  logits [T, E] of `dtype` with element
- * stride row_stride between rows, bias fp32 [E] (finite) or NULL, ids int64 / weights fp32 [T, topk].
+ * masked (never chosen; nor are experts with a NaN or -inf bias); missing experts give id -1 and weight 0.  logits
+ * [T, E] of `dtype` with element stride row_stride between rows, bias fp32 [E] or NULL (+inf counts as the
+ * largest float), ids int64 / weights fp32 [T, topk].
  * E <= 1024, n_group <= 32, topk <= 32.
  * ------------------------------------------------------------------------------------------- */
 EXL3_API int exl3_route_logits(const void* logits, int64_t dtype, int64_t T, int64_t E, int64_t row_stride,

@@ -89,6 +89,37 @@ def test_masked_logits_and_empty_rows(ext, cuda_device, G, keep):
             assert ids[0].tolist() == [-1] * 6 and w[0].tolist() == [0.0] * 6
 
 
+@pytest.mark.parametrize("G,keep", [(1, 1), (4, 2)])
+def test_masked_biases(ext, cuda_device, G, keep):
+    """A bias of -inf or NaN keeps its expert from being chosen; one of +inf puts it first."""
+    logits, bias = _logits(40, 48, torch.float32, cuda_device, seed=14)
+    bias[3], bias[20:30], bias[47] = float("nan"), -float("inf"), float("inf")
+    logits[1, 4:47] = -float("inf")                          # experts 0, 1, 2 and 47 are left
+    logits[2:20] = logits[2] + 1e-7 * logits[2:20]           # near-ties: the ranking in 64 bits
+    bias[:3] = 0.25
+    logits[2:20, :3] = 0.5
+    assert bool(bias.isnan().any())
+    masked = logits.clone()
+    masked[:, 3] = float("nan")
+    masked[:, 20:30] = -float("inf")
+    finite = bias.clone()
+    finite[3] = 0
+    finite[20:30] = 0
+    finite[47] = 1e30
+    ids, _ = check(masked, finite, 6, "sigmoid", G, keep)    # the sigmoid has no sum that a bias could change
+    r = exl3_router.LogitsRouter(6, bias=bias, n_group=G, topk_group=keep, scale=2.5)
+    got, w = r.route(logits)
+    assert torch.equal(got, ids)
+    for softmax in ("sigmoid", "softmax"):
+        got, w = exl3_router.LogitsRouter(6, softmax, bias, G, keep).route(logits)
+        chosen = got[got >= 0]
+        assert not bool(((chosen == 3) | ((chosen >= 20) & (chosen < 30))).any()) and bool(torch.isfinite(w).all())
+        assert all(len(set(row)) == len(row) for row in ([e for e in t if e >= 0] for t in got.tolist()))
+        first = (got == 47).any(1)                           # (alone in its group, it has no sum of two in row 1)
+        assert bool(first[torch.arange(40, device=cuda_device) != 1].all()) and bool(first[1]) == (G == 1)
+        assert got[1].tolist().count(-1) >= 2
+
+
 def test_near_ties_are_decided_exactly(ext, cuda_device):
     """Scores plus bias that 32 bits cannot tell apart (gaps of 1e-9 .. 1e-7 around equal sums)."""
     dev = cuda_device
