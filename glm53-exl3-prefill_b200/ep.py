@@ -70,8 +70,14 @@ def balanced_placement(counts, world: int, tile_rows: int = 256):
     return [e for r in range(world) for e in sorted(members[r])]
 
 
+def _trellis_layer(layer):
+    if getattr(layer, "w13_trellis", None) is None:
+        raise RuntimeError("expert parallelism takes trellis layers (8-bit experts run on one GPU)")
+
+
 def layer_take(layer, experts):
     """Copy of a stacked layer holding `experts` (global ids) in that order."""
+    _trellis_layer(layer)
     idx = torch.as_tensor(list(experts), dtype=torch.long, device=layer.w13_trellis.device)
     out = types.SimpleNamespace()
     for name in ("w13_trellis", "w13_suh", "w13_svh", "w2_trellis", "w2_suh", "w2_svh"):
@@ -82,6 +88,7 @@ def layer_take(layer, experts):
 
 def layer_slice(layer, e0: int, e1: int):
     """View of a stacked layer restricted to experts [e0, e1) (same attribute names and layouts)."""
+    _trellis_layer(layer)
     out = types.SimpleNamespace()
     for name in ("w13_trellis", "w13_suh", "w13_svh", "w2_trellis", "w2_suh", "w2_svh"):
         setattr(out, name, getattr(layer, name)[e0:e1])
@@ -320,6 +327,7 @@ class ExpertParallel:
             raise RuntimeError(f"{T} tokens exceed tokens_per_rank={self.tpr}")
         if tuple(ids.shape) != (T, self.topk) or tuple(weights.shape) != (T, self.topk):
             raise RuntimeError("ids / weights must be [T, topk]")
+        _trellis_layer(layer_local)
         if int(layer_local.w13_trellis.shape[0]) != self.e1 - self.e0:
             raise RuntimeError("layer_local must hold this rank's experts")
         hook("dispatch_setup")

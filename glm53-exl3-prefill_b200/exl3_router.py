@@ -48,7 +48,7 @@ class LogitsRouter:
 
     With c = score + bias: a group's score is the sum of its `group_top` largest c; the topk experts by c
     inside the `topk_group` best of `n_group` groups are chosen, best first, ties to the lower id.  Masked
-    experts (logit -inf or NaN) are never chosen; a token with fewer than topk left gets id -1, weight 0."""
+    experts (logit or bias -inf or NaN) are never chosen; a token with fewer than topk left gets id -1, weight 0."""
 
     def __init__(self, topk: int, scoring: str = "sigmoid", bias: torch.Tensor | None = None, n_group: int = 1,
                  topk_group: int = 1, group_top: int = 2, norm: bool = True, scale: float = 1.0):
@@ -74,6 +74,9 @@ def moe_prefill_from_logits(x2d: torch.Tensor, logits: torch.Tensor, router: Log
     """Hidden states [T, d] and their router logits [T, E] -> routed experts (+ the shared expert if given), fp32
     [T, d]; trellis and 8-bit layers alike.  With return_routing, also returns (ids, weights)."""
     import exl3_dense
+    experts = layer.w13_fp8 if exl3_fp8.is_fp8_layer(layer) else layer.w13_trellis
+    if logits.dim() == 2 and logits.shape[1] != experts.shape[0]:
+        raise RuntimeError("the logits and the layer disagree on the number of experts")
     ids, w = router.route(logits)
     out = exl3_dense.moe_block_prefill(x2d, ids, w, layer, shared, limit)
     return (out, ids, w) if return_routing else out

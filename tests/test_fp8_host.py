@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import b200_ext
+import ep
 import exl3_dense
 import exl3_fp8
 import exl3_router
@@ -161,6 +162,15 @@ def test_workspace_sizes_name_their_refusal(lib):
     assert "fp8_linear: invalid sizes" in lib.exl3_last_error().decode()
     assert lib.exl3_fp8_mlp_workspace(4, 256, 64) == -1
     assert "f must be a multiple of 128" in lib.exl3_last_error().decode()
+
+
+def test_layers_that_do_not_fit_are_refused():
+    L = types.SimpleNamespace(w13_fp8=torch.zeros(2, 256, 256, dtype=torch.float8_e4m3fn))
+    with pytest.raises(RuntimeError, match="number of experts"):
+        exl3_router.moe_prefill_from_logits(torch.zeros(4, 256), torch.zeros(4, 3), exl3_router.LogitsRouter(1), L, 7.0)
+    for call in (lambda: ep.layer_slice(L, 0, 1), lambda: ep.layer_take(L, [0])):
+        with pytest.raises(RuntimeError, match="trellis layers"):
+            call()
 
 
 @pytest.mark.parametrize("shape", [(128, 128), (1, 16), (200, 300), (3, 130, 256)])
