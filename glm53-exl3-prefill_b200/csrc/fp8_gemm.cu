@@ -546,6 +546,9 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
             // ============================================================ TMA producer
             Ring<FG_STAGES> st;
             int issued = 0;
+            // with a limit of zero it gives up at the first stage that is not free, and the other roles find the flag (a
+            // try_wait by itself suspends for longer than any of these waits takes)
+            const int room = p.wait_ns > 0 ? -1 : FG_STAGES;
             bool ok = true;
             for (int t = cluster; ok && t < total; t += n_clusters)
             {
@@ -565,7 +568,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 for (int kb = ti.kb0; kb < ti.kb1; ++kb, ++issued, st.next())
                 {
                     // (the first pass does not wait: a fresh barrier counts as past the phase of parity 1)
-                    ok = warp_wait(&bar_done[st.slot], st.parity ^ 1u, abort_flag, p.status, p.wait_ns);
+                    ok = issued != room && warp_wait(&bar_done[st.slot], st.parity ^ 1u, abort_flag, p.status, p.wait_ns);
                     if (!ok) break;
                     if (elect_one())
                     {
@@ -580,6 +583,11 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                     }
                     __syncwarp();
                 }
+            }
+            if (issued == room && !ok)
+            {
+                *abort_flag = 1;
+                record_error(p.status, kErrWaitTimeout);
             }
             // a stage whose MMAs are done has landed; after an abort this gives the copies in flight their time
             for (int i = issued > FG_STAGES ? issued - FG_STAGES : 0; i < issued; ++i)

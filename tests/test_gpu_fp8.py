@@ -333,3 +333,73 @@ def test_two_graphs_on_two_streams(ext, cuda_device):
     for o, e in zip(outs, eager):
         assert torch.equal(o, e)
     assert ext.read_status(dev) == 0
+
+
+@pytest.mark.parametrize("T", [1, 2, 9, 40, 300])
+def test_non_finite_tokens_stay_in_their_rows(ext, cuda_device, T):
+    """One value of a token is NaN or inf: its outputs are NaN, every other token's stay as they were."""
+    dev = cuda_device
+    E, d, f, k = 24, 256, 128, 2
+    L, S = make_layer(E, d, f, 71, dev), make_layer(1, d, f, 73, dev)
+    ids, w = (t.to(dev) for t in synth.routing("uniform", T, E, k, seed=5))
+    x = rows(T, d, torch.float32, dev, 2)
+    bad = T // 2
+    keep = torch.arange(T, device=dev) != bad
+    calls = [lambda v: exl3_fp8.fp8_linear(v, S.w13_fp8[0], S.w13_scale[0]), lambda v: exl3_fp8.fp8_mlp_prefill(v, S, LIMIT),
+             lambda v: exl3_fp8.fp8_prefill(v, ids, w, L, LIMIT)]
+    for value in (float("nan"), float("inf"), -float("inf")):
+        y = x.clone()
+        y[bad, 131] = value
+        for call in calls:
+            got = call(y)
+            assert bool(torch.isnan(got[bad]).all()) and torch.equal(got[keep], call(x)[keep])
+    big = x.clone()
+    big[bad] *= 1e30                                         # finite: the activations stop at the limit
+    assert bool(torch.isfinite(exl3_fp8.fp8_mlp_prefill(big, S, LIMIT)).all())
+
+
+@pytest.mark.parametrize("T", [1, 2, 9, 40, 300])
+def test_output_added_to_the_input(ext, cuda_device, T):
+    """x += mlp(x) in place gives what separate tensors give; a linear layer of one token refuses it."""
+    dev = cuda_device
+    E, d, k = 24, 256, 2
+    L, S = make_layer(E, d, 128, 81, dev), make_layer(1, d, 128, 83, dev)
+    w, ws = make_weight((d, d), 85, dev)
+    ids, rw = (t.to(dev) for t in synth.routing("uniform", T, E, k, seed=5))
+    x = rows(T, d, torch.float32, dev, 2)
+    calls = [lambda v, o: exl3_fp8.fp8_mlp_prefill(v, S, LIMIT, out=o), lambda v, o: exl3_fp8.fp8_prefill(v, ids, rw, L, LIMIT, out=o)]
+    if T > 1:
+        calls.append(lambda v, o: exl3_fp8.fp8_linear(v, w, ws, out=o))
+    else:
+        with pytest.raises(RuntimeError, match="overlaps x"):
+            exl3_fp8.fp8_linear(x, w, ws, out=x)
+    for call in calls:
+        want, same = call(x, x.clone()), x.clone()
+        assert call(same, same) is same and torch.equal(same, want)
+
+
+def test_products_give_up_then_recover(ext, cuda_device):
+    """With a wait limit of 0 every wait that is not over yet gives up: the tcgen05 product records a timeout, drains what
+    it issued and returns; the next calls are right.  Wide and thin tiles, stored and activated outputs."""
+    dev = cuda_device
+    # nothing waits before a CTA's five stages are full, so a tile needs more than five K blocks: here eight and more
+    # (at 400 x 1024 x 1024 K is split into parts of four blocks, and no wait gives up)
+    E, d, f, k, T = 4, 1024, 4096, 2, 400
+    L = make_layer(E, d, f, 91, dev)
+    x = rows(T, d, torch.float16, dev, 3)
+    ids, w = (t.to(dev) for t in synth.routing("uniform", T, E, k, seed=5))
+    linear = lambda: exl3_fp8.fp8_linear(x, L.w13_fp8[0], L.w13_scale[0])
+    experts = lambda: exl3_fp8.fp8_prefill(x, ids, w, L, LIMIT)
+    want = [linear(), experts()]
+    ext.read_status(dev)
+    for call, right in zip((linear, experts), want):
+        prev = ext.set_wait_limit_ns(0)
+        try:
+            call()
+            torch.cuda.synchronize()
+        finally:
+            ext.set_wait_limit_ns(prev)
+        assert ext.read_status(dev) == 1
+        assert torch.equal(call(), right) and torch.equal(call(), right)
+        torch.cuda.synchronize()
+        assert ext.read_status(dev) == 0
