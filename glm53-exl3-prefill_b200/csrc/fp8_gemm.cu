@@ -724,6 +724,11 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 }
                 tc_fence_after();
                 const uint32_t taddr = tmem + (it & 1u) * 128;
+                auto release = [&] {                        // the buffer is free: its sums are in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(tempty + (it & 1u) * 8);
+                };
                 if (!ti.thin)
                 {
                     const float x = s_sx[q][lane_in];
@@ -737,6 +742,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                         {
                             uint64_t d[8];
                             tmem_load(taddr + h * 64 + c * 16, d);
+                            if (h == 1 && c == 1) release();
                             #pragma unroll
                             for (int i = 0; i < 8; ++i) fma2(acc[h][c * 8 + i], d[i], ff);
                         }
@@ -756,6 +762,7 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                             {
                                 uint64_t d[8];
                                 tmem_load(taddr + h * 64 + c * 16, d);
+                                if (h == 1 && (c == 1 || g * 32 + 16 >= ti.rows)) release();
                                 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
                                 {
@@ -766,13 +773,9 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                             }
                         }
                 }
-                tc_fence_before();
+                else release();
                 __syncwarp();
-                if (lane == 0)
-                {
-                    mbar_arrive_cluster(tempty + (it & 1u) * 8);
-                    mbar_arrive(&bar_sempty[q]);
-                }
+                if (lane == 0) mbar_arrive(&bar_sempty[q]);
                 ++it;
                 sg.next();
             }
