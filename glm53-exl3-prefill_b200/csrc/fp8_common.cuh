@@ -101,12 +101,16 @@ template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
-// silu(min(g, L)) * clamp(u, -L, L) in fp32; NaN goes through.
+// silu(min(g, L)) * clamp(u, -L, L) in fp32; NaN goes through.  silu(g) = g / (1 + 2^(-g log2 e)) with the approximate
+// power and reciprocal (2^-22 each, and the rounding of the argument): the sum is at least 1, so nothing needs scaling, and where
+// the power overflows the quotient is the zero that it should be.
 __device__ __forceinline__ float clamped_swiglu(float g, float u, float limit)
 {
     g = g > limit ? limit : g;
     u = u > limit ? limit : (u < -limit ? -limit : u);
-    return __fdividef(g, 1.0f + __expf(-g)) * u;
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
+    return g * reciprocal(1.0f + e) * u;
 }
 
 }  // namespace fp8

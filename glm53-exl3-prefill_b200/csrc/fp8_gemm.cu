@@ -839,21 +839,16 @@ void fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
                 {
                     const float s = block_scale(__uint_as_float(mx), false), inv = reciprocal(s);
                     const int64_t r = ti.row0 + 128 * rank + lane_in;
-                    uint4* h = reinterpret_cast<uint4*>(p.h + r * p.h_stride + ti.nt * kBlock + g * 32);
+                    uint32_t w[8];
                     #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int j = 0; j < 8; ++j)
                     {
-                        uint32_t w[4];
+                        float q[4];
                         #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                        {
-                            float q[4];
-                            #pragma unroll
-                            for (int i = 0; i < 4; ++i) q[i] = quotient(act[16 * c + 4 * j + i], s, inv);
-                            w[j] = to_e4m3x2(q[0], q[1]) | to_e4m3x2(q[2], q[3]) << 16;
-                        }
-                        h[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int i = 0; i < 4; ++i) q[i] = quotient(act[4 * j + i], s, inv);
+                        w[j] = to_e4m3x2(q[0], q[1]) | to_e4m3x2(q[2], q[3]) << 16;
                     }
+                    store32(p.h + r * p.h_stride + ti.nt * kBlock + g * 32, w);     // (rows of h are 128-byte aligned)
                     if (g == 0) p.hs[r * p.hs_row + ti.nt * p.hs_blk] = s;
                 }
             }

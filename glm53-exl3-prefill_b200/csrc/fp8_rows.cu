@@ -203,18 +203,46 @@ void combine_routes_kernel(const CombineArgs p)
     if (p.accumulate)
         #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = to_float(out[i]);
-    for (int j = 0; j < p.topk; ++j)
+    // routes whose loads are in flight together; they do not wait for the ids: rows of unrouted slots exist, and what
+    // they hold is not used
+    constexpr int AHEAD = 8;
+    for (int j0 = 0; j0 < p.topk; j0 += AHEAD)
     {
-        const int64_t s = t * p.topk + j;
-        const int64_t e = p.ids_i64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + s)
-                                    : (int64_t) __ldg(reinterpret_cast<const int*>(p.ids) + s);
-        if (e < 0 || e >= p.E) continue;
-        const float w = route_weight(p.weights, p.wdtype, s);
-        const float4 v = sum_parts(p.y + s * p.y_stride + c, p.parts, p.part_stride);
-        a[0] = fmaf(w, v.x, a[0]);
-        a[1] = fmaf(w, v.y, a[1]);
-        a[2] = fmaf(w, v.z, a[2]);
-        a[3] = fmaf(w, v.w, a[3]);
+        float4 v[AHEAD];
+        bool valid[AHEAD];
+        #pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+        {
+            const int64_t s = t * p.topk + j0 + j;
+            valid[j] = j0 + j < p.topk;
+            if (valid[j]) v[j] = *reinterpret_cast<const float4*>(p.y + s * p.y_stride + c);
+        }
+        float w[AHEAD];
+        #pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+        {
+            const int64_t s = t * p.topk + j0 + j;
+            if (!valid[j]) continue;
+            const int64_t e = p.ids_i64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + s)
+                                        : (int64_t) __ldg(reinterpret_cast<const int*>(p.ids) + s);
+            valid[j] = e >= 0 && e < p.E;
+            w[j] = route_weight(p.weights, p.wdtype, s);
+        }
+        #pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+        {
+            if (!valid[j]) continue;
+            const int64_t s = t * p.topk + j0 + j;
+            for (int i = 1; i < p.parts; ++i)
+            {
+                const float4 o = *reinterpret_cast<const float4*>(p.y + s * p.y_stride + c + i * p.part_stride);
+                v[j].x += o.x; v[j].y += o.y; v[j].z += o.z; v[j].w += o.w;
+            }
+            a[0] = fmaf(w[j], v[j].x, a[0]);
+            a[1] = fmaf(w[j], v[j].y, a[1]);
+            a[2] = fmaf(w[j], v[j].z, a[2]);
+            a[3] = fmaf(w[j], v[j].w, a[3]);
+        }
     }
     #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = from_float<To>(a[i]);
