@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import threading
 
 import torch
@@ -69,6 +70,7 @@ _SIGNATURES = {
     "exl3_fp8_experts_workspace": ([_I64, _I64, _I64, _I64, _I64], _I64),
     "exl3_fp8_experts": ([_P, _I64, _I64, _I64, _I64, _P, _I32, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _F64, _P,
                           _I64, _I64, _I32, _P, _I64, _P, _P], _I32),
+    "exl3_call": ([ctypes.c_char_p], _I32),
     "exl3_ep_alloc": ([_I64, ctypes.POINTER(_P)], _I32),
     "exl3_ep_free": ([_P], _I32),
     "exl3_ep_ipc_handle": ([_P, _P], _I32),
@@ -378,13 +380,27 @@ _raw_stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
                or (lambda index: torch.cuda.current_stream(index).cuda_stream))
 
 
-def _launch(index, fn, *args):
-    """fn(*args, stream) on GPU `index` and its current stream."""
+def _packer(code, name):
+    """The arguments of an entry point (its stream last) as exl3_call's block of words."""
+    args = _SIGNATURES[name][0]
+    pack = struct.Struct("q" + "".join("d" if a is _F64 else "q" for a in args)).pack
+    return functools.partial(pack, code + 256 * len(args))
+
+
+_ROUTE_LOGITS = _packer(1, "exl3_route_logits")
+_QUANTIZE_ROWS = _packer(2, "exl3_fp8_quantize_rows")
+_LINEAR = _packer(3, "exl3_fp8_linear")
+_MLP = _packer(4, "exl3_fp8_mlp")
+_EXPERTS = _packer(5, "exl3_fp8_experts")
+
+
+def _launch(index, packer, *args):
+    """The packer's entry point with (*args, stream) on GPU `index` and its current stream."""
     if _current_device() == index:
-        rc = fn(*args, _raw_stream(index))
+        rc = load().exl3_call(packer(*args, _raw_stream(index)))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
+            rc = load().exl3_call(packer(*args, _raw_stream(index)))
     if rc:
         raise RuntimeError(load().exl3_last_error().decode(errors="replace"))
 
@@ -438,8 +454,8 @@ def route_logits(logits, bias, topk, softmax, n_group, topk_group, group_top, no
     if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (T, topk):
         _fail("route_logits: weights fp32 [T, topk]")
     index = _gpu_of(logits, bias, ids, weights)
-    _launch(index, load().exl3_route_logits, logits.data_ptr(), _WDTYPE[logits.dtype], T, E, stride,
-            None if bias is None else bias.data_ptr(), 1 if softmax else 0, n_group, topk_group, group_top, topk,
+    _launch(index, _ROUTE_LOGITS, logits.data_ptr(), _WDTYPE[logits.dtype], T, E, stride,
+            0 if bias is None else bias.data_ptr(), 1 if softmax else 0, n_group, topk_group, group_top, topk,
             1 if norm else 0, scale, ids.data_ptr(), weights.data_ptr())
 
 
@@ -452,7 +468,7 @@ def fp8_quantize_rows(x, pow2, q, scale):
         _fail("fp8_quantize_rows: scale fp32 [T, ceil(K / 128)]")
     index = _gpu_of(x, q, scale)
     s_row, s_blk = scale.stride()
-    _launch(index, load().exl3_fp8_quantize_rows, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, 1 if pow2 else 0,
+    _launch(index, _QUANTIZE_ROWS, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, 1 if pow2 else 0,
             q.data_ptr(), q.stride(0), scale.data_ptr(), s_row, s_blk)
 
 
@@ -468,7 +484,7 @@ def _workspace(index, name, *sizes):
     """(tensor, address, bytes) of the scratch a call needs, from torch's caching allocator."""
     n = _workspace_bytes(name, *sizes)
     if n == 0:
-        return None, None, 0
+        return None, 0, 0
     ws = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", index))
     return ws, ws.data_ptr(), n
 
@@ -487,7 +503,7 @@ def fp8_linear(x, w, w_scale, out, accumulate=False):
     if K % 16:
         _fail("fp8_linear: K must be a multiple of 16")
     ws, ptr, nbytes = _workspace(index, "exl3_fp8_linear_workspace", T, K, N)
-    _launch(index, load().exl3_fp8_linear, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, w.data_ptr(),
+    _launch(index, _LINEAR, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, w.data_ptr(),
             w.stride(0) if N > 1 else K, w_scale.data_ptr(), max(w_scale.stride(0), kb), N, out.data_ptr(),
             _WDTYPE[out.dtype], out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
 
@@ -516,7 +532,7 @@ def fp8_mlp(x, w13, w13_scale, w2, w2_scale, limit, out, accumulate=False):
     index = _gpu_of(x, w13, w13_scale, w2, w2_scale, out)
     _check_out(out, T, d, "fp8_mlp")
     ws, ptr, nbytes = _workspace(index, "exl3_fp8_mlp_workspace", T, d, f)
-    _launch(index, load().exl3_fp8_mlp, x.data_ptr(), _WDTYPE[x.dtype], T, d, stride, w13.data_ptr(),
+    _launch(index, _MLP, x.data_ptr(), _WDTYPE[x.dtype], T, d, stride, w13.data_ptr(),
             w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), f, limit, out.data_ptr(), _WDTYPE[out.dtype],
             out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
 
@@ -536,7 +552,7 @@ def fp8_experts(x, ids, weights, w13, w13_scale, w2, w2_scale, limit, out, accum
     index = _gpu_of(x, ids, weights, w13, w13_scale, w2, w2_scale, out)
     _check_out(out, T, d, "fp8_experts")
     ws, ptr, nbytes = _workspace(index, "exl3_fp8_experts_workspace", T, topk, E, d, f)
-    _launch(index, load().exl3_fp8_experts, x.data_ptr(), _WDTYPE[x.dtype], T, d, stride, ids.data_ptr(),
+    _launch(index, _EXPERTS, x.data_ptr(), _WDTYPE[x.dtype], T, d, stride, ids.data_ptr(),
             1 if ids.dtype == torch.int64 else 0, weights.data_ptr(), _WDTYPE[weights.dtype], topk, E, w13.data_ptr(),
             w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), f, limit, out.data_ptr(), _WDTYPE[out.dtype],
             out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))

@@ -1,6 +1,9 @@
 // capi_fp8.cu — the extern "C" boundary of routing from logits and of the 8-bit (e4m3) layers: argument
 // checks, the workspace's layout, and the order of the launches.  Nothing here allocates or synchronises.
 #include <cstdint>
+#include <cstring>
+#include <type_traits>
+#include <utility>
 
 #include <cuda_runtime.h>
 
@@ -174,6 +177,32 @@ int run_mlp(const Rows8& x, const Rows8& h, const Parts& gu, const Parts& y, int
     if (y.n > 1) return run_split(q, y, stream);
     q.out = out; q.out_stride = out_stride; q.out_dtype = (int) out_dtype; q.accumulate = accumulate;
     return launch_fp8_gemm(q, stream);
+}
+
+template <class A>
+A argument(const int64_t* word)
+{
+    if constexpr (std::is_pointer_v<A>) return reinterpret_cast<A>(*word);
+    else if constexpr (std::is_same_v<A, double>)
+    {
+        double d;
+        std::memcpy(&d, word, sizeof d);
+        return d;
+    }
+    else return static_cast<A>(*word);
+}
+
+template <class... A, size_t... I>
+int call_with(int (*fn)(A...), const int64_t* args, std::index_sequence<I...>)
+{
+    return fn(argument<A>(args + I)...);
+}
+
+template <class... A>
+int call_packed(int (*fn)(A...), const int64_t* words)
+{
+    if (words[0] >> 8 != (int64_t) sizeof...(A)) return set_error("exl3_call: wrong number of arguments");
+    return call_with(fn, words + 1, std::index_sequence_for<A...>());
 }
 
 }  // namespace
@@ -392,6 +421,21 @@ int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t
     if (rc) return rc;
     return launch_fp8_combine(b.y.p, b.y.ld, b.y.n, b.y.stride, ids, ids_is_int64 ? 1 : 0, weights, (int) weight_dtype, T,
                               (int) topk, (int) E, (int) d, accumulate ? 1 : 0, out, (int) out_dtype, out_stride, st);
+}
+
+int exl3_call(const void* words)
+{
+    const int64_t* w = static_cast<const int64_t*>(words);
+    if (!w) return set_error("exl3_call: no arguments");
+    switch (w[0] & 255)
+    {
+        case EXL3_CALL_ROUTE_LOGITS: return call_packed(exl3_route_logits, w);
+        case EXL3_CALL_FP8_QUANTIZE_ROWS: return call_packed(exl3_fp8_quantize_rows, w);
+        case EXL3_CALL_FP8_LINEAR: return call_packed(exl3_fp8_linear, w);
+        case EXL3_CALL_FP8_MLP: return call_packed(exl3_fp8_mlp, w);
+        case EXL3_CALL_FP8_EXPERTS: return call_packed(exl3_fp8_experts, w);
+        default: return set_error("exl3_call: unknown call");
+    }
 }
 
 }  // extern "C"

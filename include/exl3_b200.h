@@ -284,6 +284,12 @@ EXL3_API int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d
                               int64_t f, double limit, void* out, int64_t out_dtype, int64_t out_stride,
                               int accumulate, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 
+/* One of the five calls above from one block of 8-byte words, for bindings that pay for every argument (through ctypes
+ * 16 arguments take 2.9 us, one block 0.6): words[0] = EXL3_CALL_* + 256 * (number of arguments), then the arguments in
+ * their order, integers and addresses as int64, doubles as they are. */
+enum { EXL3_CALL_ROUTE_LOGITS = 1, EXL3_CALL_FP8_QUANTIZE_ROWS, EXL3_CALL_FP8_LINEAR, EXL3_CALL_FP8_MLP, EXL3_CALL_FP8_EXPERTS };
+EXL3_API int exl3_call(const void* words);
+
 /* ---------------------------------------------------------------------------------------------
  * Expert parallelism.  No reference counterpart: the reference refuses expert-parallel layers
  * (kernel/exl3_grouped_runtime.py:96-98, `layer.expert_map is not None` falls back).  One process per

@@ -173,6 +173,26 @@ def test_layers_that_do_not_fit_are_refused():
             call()
 
 
+def test_packed_calls_reach_their_entry_points(lib):
+    """Every argument of a packed call arrives: the refusals are those of the entry point itself."""
+    def call(packer, *args):
+        return lib.exl3_call(packer(*args))
+    ok = [4096, 0, 4, 16, 16, 0, 0, 1, 1, 1, 4, 1, 1.0, 4096, 4096, 0]
+    for i, bad, text in [(1, 3, "float32, float16"), (3, 1025, "too many experts"), (4, 15, "rows overlap"), (7, 3, "divide"),
+                         (10, 17, "topk must be"), (12, float("inf"), "scale must be finite"), (13, 0, "CUDA")]:
+        refused(lib, call(b200_ext._ROUTE_LOGITS, *[bad if j == i else a for j, a in enumerate(ok)]), text)
+    assert call(b200_ext._ROUTE_LOGITS, *[0 if j == 2 else a for j, a in enumerate(ok)]) == 0
+    refused(lib, call(b200_ext._QUANTIZE_ROWS, 4096, 1, 4, 256, 256, 0, 4096, 255, 4096, 2, 1, 0), "output rows overlap")
+    refused(lib, call(b200_ext._LINEAR, 4096, 1, 4, 256, 256, 4096, 256, 4096, 2, 64, 4096, 0, 64, 0, 4096, 16, 0, 0), "workspace must")
+    refused(lib, call(b200_ext._MLP, 4096, 1, 4, 256, 256, 4096, 4096, 4096, 4096, 128, -1.0, 4096, 0, 256, 0, 4096, 16, 0, 0),
+            "limit must be positive")
+    refused(lib, call(b200_ext._EXPERTS, 4096, 1, 4, 256, 256, 4096, 1, 4096, 0, 2, 8, 4096, 4096, 4096, 4096, 128, 7.0, 4096, 0,
+                      256, 0, 4096, 16, 0, 0), "workspace must hold")
+    refused(lib, lib.exl3_call(None), "no arguments")
+    refused(lib, lib.exl3_call((1 + 256 * 3).to_bytes(8, "little") + bytes(64)), "number of arguments")
+    refused(lib, lib.exl3_call((99).to_bytes(8, "little")), "unknown call")
+
+
 @pytest.mark.parametrize("shape", [(128, 128), (1, 16), (200, 300), (3, 130, 256)])
 def test_quantize_weight(shape):
     w = torch.randn(*shape, generator=torch.Generator().manual_seed(1))
