@@ -396,11 +396,12 @@ _EXPERTS = _packer(5, "exl3_fp8_experts")
 
 def _launch(index, packer, *args):
     """The packer's entry point with (*args, stream) on GPU `index` and its current stream."""
+    lib = _lib or load()
     if _current_device() == index:
-        rc = load().exl3_call(packer(*args, _raw_stream(index)))
+        rc = lib.exl3_call(packer(*args, _raw_stream(index)))
     else:
         with torch.cuda.device(index):
-            rc = load().exl3_call(packer(*args, _raw_stream(index)))
+            rc = lib.exl3_call(packer(*args, _raw_stream(index)))
     if rc:
         raise RuntimeError(load().exl3_last_error().decode(errors="replace"))
 
@@ -426,8 +427,9 @@ def _gpu_of(first, *others):
 
 
 def _rows_of(x, what):
-    """(rows, columns, row stride) of a 2-D tensor with contiguous, separate rows of a dtype the kernels read."""
-    if x.dtype not in _WDTYPE:
+    """(rows, columns, row stride, dtype code) of a 2-D tensor with contiguous, separate rows that the kernels read."""
+    code = _WDTYPE.get(x.dtype)
+    if code is None:
         _fail(f"{what} must be {_DTYPE_NAMES}")
     if x.dim() != 2:
         _fail(f"{what} must be [rows, columns]")
@@ -435,41 +437,46 @@ def _rows_of(x, what):
     stride, one = x.stride()
     if (cols > 1 and one != 1) or (rows > 1 and stride < cols):
         _fail(f"{what} must be [rows, columns] with contiguous, separate rows")
-    return rows, cols, stride
+    return rows, cols, stride, code
 
 
-def _check_out(out, T, N, what):
-    if (out.dtype not in _WDTYPE or out.dim() != 2 or out.shape[0] != T or out.shape[1] != N
-            or (N > 1 and out.stride(1) != 1)):
+def _output(out, out_dtype, T, N, device, what):
+    """(out, its dtype code, its row stride): a new [T, N] tensor, or the caller's after its checks."""
+    if out is None:
+        code = _WDTYPE.get(out_dtype)
+        if code is None:
+            _fail(f"{what}: out_dtype must be {_DTYPE_NAMES}")
+        return torch.empty(T, N, dtype=out_dtype, device=device), code, N
+    if (out.dtype not in _WDTYPE or out.dim() != 2 or out.shape != (T, N) or (N > 1 and out.stride(1) != 1)):
         _fail(f"{what}: out [{T}, {N}] ({_DTYPE_NAMES}, contiguous rows) on the input's device")
+    return out, _WDTYPE[out.dtype], out.stride(0)
 
 
-def route_logits(logits, bias, topk, softmax, n_group, topk_group, group_top, norm, scale, ids, weights):
-    """exl3_route_logits: logits [T, E] -> ids int64 / weights fp32 [T, topk]."""
-    T, E, stride = _rows_of(logits, "route_logits: logits")
+def route_logits(logits, bias, topk, softmax, n_group, topk_group, group_top, norm, scale):
+    """exl3_route_logits: logits [T, E] -> (ids int64, weights fp32) [T, topk]."""
+    T, E, stride, code = _rows_of(logits, "route_logits: logits [T, E]")
     if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous() or bias.numel() != E):
         _fail("route_logits: bias fp32 [E]")
-    if ids.dtype != torch.int64 or not ids.is_contiguous() or ids.shape != (T, topk):
-        _fail("route_logits: ids int64 [T, topk]")
-    if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (T, topk):
-        _fail("route_logits: weights fp32 [T, topk]")
-    index = _gpu_of(logits, bias, ids, weights)
-    _launch(index, _ROUTE_LOGITS, logits.data_ptr(), _WDTYPE[logits.dtype], T, E, stride,
-            0 if bias is None else bias.data_ptr(), 1 if softmax else 0, n_group, topk_group, group_top, topk,
-            1 if norm else 0, scale, ids.data_ptr(), weights.data_ptr())
+    index = _gpu_of(logits, bias)
+    device = logits.device
+    ids = torch.empty(T, topk, dtype=torch.int64, device=device)
+    weights = torch.empty(T, topk, dtype=torch.float32, device=device)
+    _launch(index, _ROUTE_LOGITS, logits.data_ptr(), code, T, E, stride, 0 if bias is None else bias.data_ptr(), softmax,
+            n_group, topk_group, group_top, topk, norm, scale, ids.data_ptr(), weights.data_ptr())
+    return ids, weights
 
 
-def fp8_quantize_rows(x, pow2, q, scale):
-    """exl3_fp8_quantize_rows: x [T, K] -> q e4m3 [T, K], scale fp32 [T, ceil(K / 128)] (any strides)."""
-    T, K, stride = _rows_of(x, "fp8_quantize_rows: x")
-    if q.dtype != _E4M3 or q.shape != (T, K) or (K > 1 and q.stride(1) != 1):
-        _fail("fp8_quantize_rows: q e4m3 [T, K]")
-    if scale.dtype != torch.float32 or scale.shape != (T, -(-K // 128)):
-        _fail("fp8_quantize_rows: scale fp32 [T, ceil(K / 128)]")
-    index = _gpu_of(x, q, scale)
-    s_row, s_blk = scale.stride()
-    _launch(index, _QUANTIZE_ROWS, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, 1 if pow2 else 0,
-            q.data_ptr(), q.stride(0), scale.data_ptr(), s_row, s_blk)
+def fp8_quantize_rows(x, pow2):
+    """exl3_fp8_quantize_rows: x [T, K] -> (q e4m3 [T, K], scale fp32 [T, ceil(K / 128)])."""
+    T, K, stride, code = _rows_of(x, "quantize_rows: x [T, K]")
+    index = _gpu_of(x)
+    device, blocks = x.device, -(-K // 128)
+    q = torch.empty(T, K, dtype=_E4M3, device=device)
+    scale = torch.empty(T, blocks, dtype=torch.float32, device=device)
+    if T and K:
+        _launch(index, _QUANTIZE_ROWS, x.data_ptr(), code, T, K, stride, 1 if pow2 else 0, q.data_ptr(), K,
+                scale.data_ptr(), blocks, 1)
+    return q, scale
 
 
 @functools.lru_cache(maxsize=1024)
@@ -489,29 +496,42 @@ def _workspace(index, name, *sizes):
     return ws, ws.data_ptr(), n
 
 
-def fp8_linear(x, w, w_scale, out, accumulate=False):
-    """exl3_fp8_linear: out [T, N] (+)= quantised(x [T, K]) . w^T, w e4m3 [N, K], w_scale fp32 [N/128, K/128]."""
-    T, K, stride = _rows_of(x, "fp8_linear: x")
-    if w.dtype != _E4M3 or w.dim() != 2 or w.shape[1] != K or (K > 1 and w.stride(1) != 1):
+def fp8_linear(x, w, w_scale, out=None, out_dtype=torch.float32):
+    """exl3_fp8_linear: quantised(x [T, K]) . w^T as a new [T, N] of out_dtype, or added into out; w e4m3 [N, K], w_scale
+    fp32 [N/128, K/128]."""
+    T, K, stride, code = _rows_of(x, "fp8_linear: x")
+    if w.dtype != _E4M3 or w.dim() != 2:
         _fail("fp8_linear: weight e4m3 [N, K] with contiguous rows")
-    N, kb = w.shape[0], -(-K // 128)
-    if (w_scale.dtype != torch.float32 or w_scale.shape != (-(-N // 128), kb) or (kb > 1 and w_scale.stride(1) != 1)
-            or (N > 128 and w_scale.stride(0) < kb)):
-        _fail("fp8_linear: weight_scale fp32 [ceil(N/128), ceil(K/128)] with contiguous, separate rows")
-    index = _gpu_of(x, w, w_scale, out)
-    _check_out(out, T, N, "fp8_linear")
+    N, w_cols = w.shape
+    w_row, w_one = w.stride()
+    if w_cols != K:
+        _fail("fp8_linear: K mismatch between x [T, K] and weight [N, K]")
+    if K > 1 and w_one != 1:
+        _fail("fp8_linear: weight e4m3 [N, K] with contiguous rows")
     if K % 16:
         _fail("fp8_linear: K must be a multiple of 16")
+    kb = -(-K // 128)
+    if w_scale.dtype != torch.float32 or w_scale.shape != (-(-N // 128), kb):
+        _fail("fp8_linear: weight_scale fp32 [ceil(N/128), ceil(K/128)]")
+    s_row, s_one = w_scale.stride()
+    if (kb > 1 and s_one != 1) or (N > 128 and s_row < kb):
+        _fail("fp8_linear: weight_scale [ceil(N/128), ceil(K/128)] with contiguous, separate rows")
+    index = _gpu_of(x, w, w_scale, out)
+    accumulate = out is not None
+    out, out_code, out_stride = _output(out, out_dtype, T, N, x.device, "fp8_linear")
     ws, ptr, nbytes = _workspace(index, "exl3_fp8_linear_workspace", T, K, N)
-    _launch(index, _LINEAR, x.data_ptr(), _WDTYPE[x.dtype], T, K, stride, w.data_ptr(),
-            w.stride(0) if N > 1 else K, w_scale.data_ptr(), max(w_scale.stride(0), kb), N, out.data_ptr(),
-            _WDTYPE[out.dtype], out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
+    _launch(index, _LINEAR, x.data_ptr(), code, T, K, stride, w.data_ptr(), w_row if N > 1 else K, w_scale.data_ptr(),
+            s_row if N > 128 else kb, N, out.data_ptr(), out_code, out_stride, accumulate, ptr, nbytes, _status_ptr(index))
+    return out
 
 
 def _check_fp8_layer(w13, s13, w2, s2, d, what):
-    if w13.dtype != _E4M3 or w13.dim() != 3 or w13.shape[2] != d or w13.shape[1] % 256 or not w13.is_contiguous():
+    if w13.dtype != _E4M3 or w13.dim() != 3 or not w13.is_contiguous():
         _fail(f"{what}: w13_fp8 e4m3 [E, 2f, d], f a multiple of 128")
-    E, f = w13.shape[0], w13.shape[1] // 2
+    E, f2, cols = w13.shape
+    if cols != d or f2 % 256:
+        _fail(f"{what}: w13_fp8 e4m3 [E, 2f, d], f a multiple of 128")
+    f = f2 // 2
     if d % 128:
         _fail(f"{what}: d must be a multiple of 128")
     if w2.dtype != _E4M3 or w2.shape != (E, d, f) or not w2.is_contiguous():
@@ -523,39 +543,45 @@ def _check_fp8_layer(w13, s13, w2, s2, d, what):
     return E, f
 
 
-def fp8_mlp(x, w13, w13_scale, w2, w2_scale, limit, out, accumulate=False):
-    """exl3_fp8_mlp: out [T, d] (+)= the gated MLP stored as one expert ([1, 2f, d], [1, d, f]) of x [T, d]."""
-    T, d, stride = _rows_of(x, "fp8_mlp: x")
+def fp8_mlp(x, w13, w13_scale, w2, w2_scale, limit, out=None, out_dtype=torch.float32):
+    """exl3_fp8_mlp: the gated MLP stored as one expert ([1, 2f, d], [1, d, f]) of x [T, d] as a new [T, d] of out_dtype, or
+    added into out."""
+    T, d, stride, code = _rows_of(x, "fp8_mlp: x")
     E, f = _check_fp8_layer(w13, w13_scale, w2, w2_scale, d, "fp8_mlp")
     if E != 1:
         _fail("fp8_mlp: the MLP must be stored as one expert ([1, ...] tensors)")
     index = _gpu_of(x, w13, w13_scale, w2, w2_scale, out)
-    _check_out(out, T, d, "fp8_mlp")
+    accumulate = out is not None
+    out, out_code, out_stride = _output(out, out_dtype, T, d, x.device, "fp8_mlp")
     ws, ptr, nbytes = _workspace(index, "exl3_fp8_mlp_workspace", T, d, f)
-    _launch(index, _MLP, x.data_ptr(), _WDTYPE[x.dtype], T, d, stride, w13.data_ptr(),
-            w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), f, limit, out.data_ptr(), _WDTYPE[out.dtype],
-            out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
+    _launch(index, _MLP, x.data_ptr(), code, T, d, stride, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(),
+            w2_scale.data_ptr(), f, limit, out.data_ptr(), out_code, out_stride, accumulate, ptr, nbytes, _status_ptr(index))
+    return out
 
 
-def fp8_experts(x, ids, weights, w13, w13_scale, w2, w2_scale, limit, out, accumulate=False):
-    """exl3_fp8_experts: out [T, d] (+)= sum_j weights[t, j] * mlp_{ids[t, j]}(x[t]) over e4m3 experts."""
-    T, d, stride = _rows_of(x, "fp8_experts: x")
+def fp8_experts(x, ids, weights, w13, w13_scale, w2, w2_scale, limit, out=None, out_dtype=torch.float32):
+    """exl3_fp8_experts: sum_j weights[t, j] * mlp_{ids[t, j]}(x[t]) over e4m3 experts as a new [T, d] of out_dtype, or
+    added into out."""
+    T, d, stride, code = _rows_of(x, "fp8_experts: x")
     E, f = _check_fp8_layer(w13, w13_scale, w2, w2_scale, d, "fp8_experts")
     if ids.dtype != torch.int64 and ids.dtype != torch.int32:
         _fail("ids must be int64 or int32")
-    if weights.dtype not in _WDTYPE:
+    weight_code = _WDTYPE.get(weights.dtype)
+    if weight_code is None:
         _fail(f"weights must be {_DTYPE_NAMES}")
-    if (ids.dim() != 2 or ids.shape[0] != T or not ids.is_contiguous() or not weights.is_contiguous()
-            or weights.shape != ids.shape):
+    shape = ids.shape
+    if (len(shape) != 2 or shape[0] != T or not ids.is_contiguous() or not weights.is_contiguous()
+            or weights.shape != shape):
         _fail("ids / weights must be contiguous [T, topk]")
-    topk = ids.shape[1]
+    topk = shape[1]
     index = _gpu_of(x, ids, weights, w13, w13_scale, w2, w2_scale, out)
-    _check_out(out, T, d, "fp8_experts")
+    accumulate = out is not None
+    out, out_code, out_stride = _output(out, out_dtype, T, d, x.device, "fp8_experts")
     ws, ptr, nbytes = _workspace(index, "exl3_fp8_experts_workspace", T, topk, E, d, f)
-    _launch(index, _EXPERTS, x.data_ptr(), _WDTYPE[x.dtype], T, d, stride, ids.data_ptr(),
-            1 if ids.dtype == torch.int64 else 0, weights.data_ptr(), _WDTYPE[weights.dtype], topk, E, w13.data_ptr(),
-            w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), f, limit, out.data_ptr(), _WDTYPE[out.dtype],
-            out.stride(0), 1 if accumulate else 0, ptr, nbytes, _status_ptr(index))
+    _launch(index, _EXPERTS, x.data_ptr(), code, T, d, stride, ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0,
+            weights.data_ptr(), weight_code, topk, E, w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(),
+            w2_scale.data_ptr(), f, limit, out.data_ptr(), out_code, out_stride, accumulate, ptr, nbytes, _status_ptr(index))
+    return out
 
 
 # ------------------------------------------------------------------------------------ expert parallelism

@@ -34,14 +34,7 @@ def is_fp8_layer(layer) -> bool:
 def quantize_rows(x2d: torch.Tensor, pow2: bool = False):
     """x2d [T, K] (fp32, fp16, bf16; rows may be strided) -> (q e4m3 [T, K], scale fp32 [T, ceil(K / 128)]).
     pow2 takes the least power of two at or above amax / 448 as the scale."""
-    if x2d.dim() != 2:
-        raise RuntimeError("quantize_rows: x must be [T, K]")
-    T, K = x2d.shape
-    q = torch.empty(T, K, dtype=torch.float8_e4m3fn, device=x2d.device)
-    scale = torch.empty(T, -(-K // BLOCK), dtype=torch.float32, device=x2d.device)
-    if T and K:
-        b200_ext.fp8_quantize_rows(x2d, pow2, q, scale)
-    return q, scale
+    return b200_ext.fp8_quantize_rows(x2d, pow2)
 
 
 def quantize_weight(w: torch.Tensor):
@@ -64,34 +57,20 @@ def fp8_linear(x2d: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tens
     """x2d [T, K], weight e4m3 [N, K], weight_scale fp32 [ceil(N/128), ceil(K/128)] -> x W^T [T, N] as out_dtype
     (float32, float16 or bfloat16), or added into `out` if given.  K must be a multiple of 16; with one token `out`
     may not overlap x (refused)."""
-    if x2d.dim() != 2 or weight.dim() != 2 or x2d.size(1) != weight.size(1):
-        raise RuntimeError("fp8_linear: K mismatch between x [T, K] and weight [N, K]")
-    accumulate = out is not None
-    if out is None:
-        out = torch.empty(x2d.size(0), weight.size(0), dtype=out_dtype, device=x2d.device)
-    b200_ext.fp8_linear(x2d, weight, weight_scale, out, accumulate)
-    return out
+    return b200_ext.fp8_linear(x2d, weight, weight_scale, out, out_dtype)
 
 
 def fp8_mlp_prefill(x2d: torch.Tensor, mlp, limit: float, out: torch.Tensor | None = None,
                     out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """A gated MLP in the layer layout with one expert -> [T, d] (added into `out` if given)."""
-    accumulate = out is not None
-    if out is None:
-        out = torch.empty(x2d.shape, dtype=out_dtype, device=x2d.device)
-    b200_ext.fp8_mlp(x2d, mlp.w13_fp8, mlp.w13_scale, mlp.w2_fp8, mlp.w2_scale, float(limit), out, accumulate)
-    return out
+    return b200_ext.fp8_mlp(x2d, mlp.w13_fp8, mlp.w13_scale, mlp.w2_fp8, mlp.w2_scale, float(limit), out, out_dtype)
 
 
 def fp8_prefill(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, layer, limit: float,
                 out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """x2d [T, d], ids [T, topk] (int64 or int32; ids outside [0, E) add nothing), weights [T, topk]
     -> sum_j weights[t, j] * mlp_{ids[t, j]}(x[t]) as out_dtype [T, d], or added into `out` if given."""
-    accumulate = out is not None
-    if out is None:
-        out = torch.empty(x2d.shape, dtype=out_dtype, device=x2d.device)
-    if ids.dim() == 2 and ids.size(1) == 0:
-        return out if accumulate else out.zero_()
-    b200_ext.fp8_experts(x2d, ids.contiguous(), weights.contiguous(), layer.w13_fp8, layer.w13_scale, layer.w2_fp8,
-                         layer.w2_scale, float(limit), out, accumulate)
-    return out
+    if ids.dim() == 2 and ids.shape[1] == 0:
+        return torch.zeros(x2d.shape, dtype=out_dtype, device=x2d.device) if out is None else out
+    return b200_ext.fp8_experts(x2d, ids.contiguous(), weights.contiguous(), layer.w13_fp8, layer.w13_scale, layer.w2_fp8,
+                                layer.w2_scale, float(limit), out, out_dtype)

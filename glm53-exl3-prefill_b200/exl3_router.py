@@ -60,13 +60,8 @@ class LogitsRouter:
 
     def route(self, logits: torch.Tensor):
         """logits [T, E] (fp32, fp16 or bf16; rows may be strided) -> (ids int64 [T, topk], weights fp32 [T, topk])."""
-        if logits.dim() != 2:
-            raise RuntimeError("LogitsRouter: logits must be [T, E]")
-        ids = torch.empty(logits.shape[0], self.topk, dtype=torch.int64, device=logits.device)
-        w = torch.empty(logits.shape[0], self.topk, dtype=torch.float32, device=logits.device)
-        b200_ext.route_logits(logits, self.bias, self.topk, self.softmax, self.n_group, self.topk_group,
-                              self.group_top, self.norm, self.scale, ids, w)
-        return ids, w
+        return b200_ext.route_logits(logits, self.bias, self.topk, self.softmax, self.n_group, self.topk_group,
+                                     self.group_top, self.norm, self.scale)
 
 
 def moe_prefill_from_logits(x2d: torch.Tensor, logits: torch.Tensor, router: LogitsRouter, layer, limit: float,
