@@ -113,7 +113,7 @@ ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_
 }
 
 // Routes whose products each read their expert's weights for themselves (fp8_small.cu), activations [R, f] in the workspace.
-// With 288 experts of 4096 x 1536 (every route another expert), 8 / 16 / 32 / 64 routes: 40 / 71 / 125 / 257 us, and 58 / 95 /
+// With 288 experts of 4096 x 1536 (every route another expert), 8 / 16 / 32 / 64 routes: 39 / 72 / 126 / 257 us, and 58 / 95 /
 // 138 / 203 us by the tiles of fp8_gemm.cu; where routes share experts the tiles read the weights once, hence the second bound.
 bool few_routes(int64_t R, int64_t E) { return R <= 32 && R <= 2 * E; }
 

@@ -12,6 +12,8 @@ using namespace fp8;
 //     q[r, k] = e4m3(x[r, k] / s[r, k / 128])       b = k / 128
 // bound by bytes: a row is read once (2 or 4 bytes a value) and written once (1 byte).  Eight lanes hold a block,
 // 16 values each, so loads are whole 32-byte sectors, the store is 16 bytes a lane, and a block's maximum is three shuffles.
+// 8192 x 12288: fp16 to powers of two 53 us (47 by bytes), bf16 with exact scales 72 us, where the seven operations of quotient()
+// for every value share the bound with the bytes.
 struct QuantArgs {
     const void* x;
     int64_t x_stride;                // elements
@@ -153,7 +155,8 @@ void gather_rows_kernel(const GatherArgs p)
 
 // ------------------------------------------------------------------------------------ sum over a token's routes
 //     out[t] = (accumulate ? out[t] : 0) + sum over j ascending, ids[t, j] in [0, E), of w[t, j] * y[t * topk + j]
-// in fp32 and a fixed order (no atomics), rounded once to out's type.  Bound by reading y.
+// in fp32 and a fixed order (no atomics), rounded once to out's type.  Bound by reading y, which is fp32 so that a result has one
+// rounding: 65536 rows of 4096 (1.07 GB, part of it still to be written back) take 270 us.
 struct CombineArgs {
     const float* y;
     int64_t y_stride;

@@ -17,7 +17,7 @@
 // knows its two best; each of the topk rounds is two warp-wide integer reductions (the largest key, then the lowest
 // expert that holds it), after which the owner moves up its second best and only looks at its keys again when that is
 // gone too.  The bytes of the logits (33 MB for 32768 tokens of 256 experts, 5 us) bound it in principle; the instructions do
-// in fact, about 450 a token.
+// in fact, about 1100 a token: 8192 tokens of 288 experts take 14.4 us (1.6 by bytes), 32768 of 256 in 8 groups 56 us.
 //
 // The choice is the one that exact arithmetic makes.  Without a bias both score functions grow with the
 // logit, so experts are ranked by the logits themselves.  With a bias, scores in 32 bits rank them, and where two scores
