@@ -403,3 +403,26 @@ def test_products_give_up_then_recover(ext, cuda_device):
         assert torch.equal(call(), right) and torch.equal(call(), right)
         torch.cuda.synchronize()
         assert ext.read_status(dev) == 0
+
+
+def test_offsets_past_32_bits(ext, cuda_device):
+    """The last rows of inputs, outputs and workspaces of more than 2^31 elements."""
+    dev = cuda_device
+    T, N = 70000, 32768                                      # 2.3e9 outputs
+    w, ws = make_weight((N, 128), 101, dev)
+    x = rows(T, 128, torch.float16, dev, 4)
+    out = exl3_fp8.fp8_linear(x, w, ws, out_dtype=torch.float16)
+    check_linear(x[-5:], w, ws, torch.float16, out[-5:])
+    q, s = exl3_fp8.quantize_rows(out)                       # 2.3e9 inputs
+    q1, s1 = exl3_fp8.quantize_rows(out[-5:])
+    assert torch.equal(q[-5:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[-5:], s1)
+    del out, q, s
+    d, f, k = 8192, 128, 4                                   # 2.3e9 values in the routes' rows
+    L = make_layer(3, d, f, 103, dev)
+    ids, rw = (t.to(dev) for t in synth.routing("uniform", T, 3, k - 1, seed=5))
+    ids, rw = torch.cat([ids, ids[:, :1]], 1), torch.cat([rw, rw[:, :1]], 1)
+    x = rows(T, d, torch.bfloat16, dev, 6)
+    got = exl3_fp8.fp8_prefill(x, ids, rw, L, LIMIT, out_dtype=torch.bfloat16)
+    # (half a bf16 step on top: 2^-8)
+    assert rel(got[-6:], ref_experts(x[-6:], ids[-6:], rw[-6:], L)) <= MLP_REL + 2.0 ** -8
+    assert ext.read_status(dev) == 0

@@ -173,3 +173,13 @@ def test_moe_from_logits_is_the_block_on_its_routing(ext, cuda_device):
     out, ids, w = exl3_router.moe_prefill_from_logits(x, logits, r, layer, 7.0, return_routing=True)
     ref = exl3_dense.moe_block_prefill(x, ids, w, layer, None, 7.0)
     assert float((out - ref).norm() / ref.norm()) < 1e-6      # the trellis down stage adds in any order
+
+
+def test_offsets_past_32_bits(ext, cuda_device):
+    dev = cuda_device
+    T, E = 9_000_000, 256                                    # 2.3e9 logits
+    logits = torch.empty(T, E, dtype=torch.bfloat16, device=dev).normal_(generator=torch.Generator(device=dev).manual_seed(3))
+    ids, w = exl3_router.LogitsRouter(2).route(logits)
+    tail_ids, tail_w = exl3_router.LogitsRouter(2).route(logits[-7:])
+    assert torch.equal(ids[-7:], tail_ids) and torch.equal(w[-7:], tail_w)
+    check(logits[-7:], None, 2)
