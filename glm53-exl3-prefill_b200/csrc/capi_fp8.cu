@@ -117,6 +117,16 @@ ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_
 // 138 / 203 us by the tiles of fp8_gemm.cu; where routes share experts the tiles read the weights once, hence the second bound.
 bool few_routes(int64_t R, int64_t E) { return R <= 32 && R <= 2 * E; }
 
+// Tokens whose product streams the weights through fp8_small.cu rather than in tiles.  Up to 8 tokens it is never slower: 6.5
+// against 14.0 us for 4096 x 4096, 23.4 against 24.3 for 24576 x 4096, 14.5 against 17.8 for 2048 x 16384.  9..16 tokens take
+// twice the instructions: 9.6 against 15.0 us for 4096 x 4096 and 16.4 against 16.8 for 8192 x 4096, but 22.1 against 19.2 for
+// 12288 x 4096, and 28.7 against 18.4 for 2048 x 16384, whose rows are long and few.
+bool few_tokens(int64_t T, int64_t N, int64_t K)
+{
+    return T <= 8 || (T <= kFp8FewTokens && N * K <= (1 << 25) && K <= 2 * N);
+}
+bool few_mlp_tokens(int64_t T, int64_t d, int64_t f) { return few_tokens(T, 2 * f, d) && few_tokens(T, d, f); }
+
 int check_rows(const char* what, int64_t dtype, int64_t rows, int64_t K, int64_t stride)
 {
     if (!is_dtype(dtype)) return set_error("%s: unknown dtype", what);
@@ -254,7 +264,7 @@ int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K, int64_t N)
     if (T <= 1) return 0;                               // one row is quantised on the way
     Carver c{nullptr};
     take_rows(c, T, K);
-    if (T > kFp8FewTokens) take_parts(c, T, 1, N, K);
+    if (!few_tokens(T, N, K)) take_parts(c, T, 1, N, K);
     return c.used;
 }
 
@@ -292,7 +302,7 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     p.sw = w_scale; p.sw_n = w_scale_stride; p.sw_expert = 0;
     p.out = out; p.out_stride = out_stride; p.out_dtype = (int) out_dtype; p.accumulate = accumulate ? 1 : 0;
     p.status = status;
-    if (T <= kFp8FewTokens) return launch_fp8_linear_tokens(p, as_stream(stream));
+    if (few_tokens(T, N, K)) return launch_fp8_linear_tokens(p, as_stream(stream));
     const Parts parts = take_parts(c, T, 1, N, K);
     if (parts.n == 1) return launch_fp8_gemm(p, as_stream(stream));
     if ((rc = run_split(p, parts, as_stream(stream)))) return rc;
@@ -304,12 +314,13 @@ int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f)
 {
     if (check_experts_shape("fp8_mlp", T, 1, 1, d, f)) return -1;
     Carver c{nullptr};
-    if (few_routes(T, 1)) c.take<float>(T * f);
-    if (few_routes(T, 1)) return c.used;
     take_rows(c, T, d);
     take_rows(c, T, f);
-    if (T <= kFp8FewTokens) c.take<float>(T * 2 * f);
-    if (T <= kFp8FewTokens) return c.used;
+    if (few_mlp_tokens(T, d, f))
+    {
+        c.take<float>(T * 2 * f);
+        return c.used;
+    }
     take_parts(c, T, 1, 2 * f, d);
     take_parts(c, T, 1, d, f);
     return c.used;
@@ -330,12 +341,8 @@ int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_s
     if (!aligned16(workspace) || workspace_bytes < exl3_fp8_mlp_workspace(T, d, f))
         return set_error("fp8_mlp: workspace must hold exl3_fp8_mlp_workspace() bytes");
     Carver c{static_cast<uint8_t*>(workspace)};
-    if (few_routes(T, 1))
-        return launch_fp8_experts_small(x, (int) dtype, (int) T, (int) d, x_stride, nullptr, 0, nullptr, 0, 1, 1, w13,
-                                        w13_scale, w2, w2_scale, (int) f, (float) limit, c.take<float>(T * f), out,
-                                        (int) out_dtype, out_stride, accumulate ? 1 : 0, as_stream(stream));
     const Rows8 xr = take_rows(c, T, d), hr = take_rows(c, T, f);
-    if (T <= kFp8FewTokens)
+    if (few_mlp_tokens(T, d, f))
     {
         // the same four steps by the kernels for few tokens: rows, gate | up sums, activations, down
         float* sums = c.take<float>(T * 2 * f);

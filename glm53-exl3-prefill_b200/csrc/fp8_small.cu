@@ -318,14 +318,12 @@ struct SmallExpertArgs {
 
 __device__ __forceinline__ int64_t route_expert(const SmallExpertArgs& p, int64_t slot)
 {
-    if (!p.ids) return 0;                                           // a plain MLP: one expert, weight 1
     return p.ids_i64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + slot)
                      : (int64_t) __ldg(reinterpret_cast<const int*>(p.ids) + slot);
 }
 
 __device__ __forceinline__ float weight_of(const SmallExpertArgs& p, int64_t slot)
 {
-    if (!p.weights) return 1.0f;
     if (p.wdtype == 0) return __ldg(reinterpret_cast<const float*>(p.weights) + slot);
     if (p.wdtype == 1) return __half2float(reinterpret_cast<const __half*>(p.weights)[slot]);
     return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.weights)[slot]);

@@ -426,3 +426,18 @@ def test_offsets_past_32_bits(ext, cuda_device):
     # (half a bf16 step on top: 2^-8)
     assert rel(got[-6:], ref_experts(x[-6:], ids[-6:], rw[-6:], L)) <= MLP_REL + 2.0 ** -8
     assert ext.read_status(dev) == 0
+
+
+@pytest.mark.parametrize("T", [8, 9, 16, 17])
+def test_both_sides_of_the_rule_for_few_tokens(ext, cuda_device, T):
+    """9..16 tokens take one path or the other by the weight's shape: long rows (K > 2 N), and square ones."""
+    dev = cuda_device
+    for N, K in ((100, 1024), (512, 512)):
+        w, ws = make_weight((N, K), 111, dev)
+        x = rows(T, K, torch.bfloat16, dev, 2)
+        check_linear(x, w, ws, torch.bfloat16, exl3_fp8.fp8_linear(x, w, ws, out_dtype=torch.bfloat16))
+    for d, f in ((1280, 256), (256, 640), (512, 512)):
+        L = make_layer(1, d, f, 113, dev)
+        x = rows(T, d, torch.bfloat16, dev, 3)
+        assert rel(exl3_fp8.fp8_mlp_prefill(x, L, LIMIT), ref_mlp(x, L, 0)) <= MLP_REL
+    assert ext.read_status(dev) == 0
