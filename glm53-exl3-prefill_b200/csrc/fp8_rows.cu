@@ -12,7 +12,7 @@ using namespace fp8;
 //     q[r, k] = e4m3(x[r, k] / s[r, k / 128])       b = k / 128
 // bound by bytes: a row is read once (2 or 4 bytes a value) and written once (1 byte).  Eight lanes hold a block,
 // 16 values each, so loads are whole 32-byte sectors, the store is 16 bytes a lane, and a block's maximum is three shuffles.
-// 8192 x 12288: fp16 to powers of two 53 us (47 by bytes), bf16 with exact scales 72 us, where the seven operations of quotient()
+// 8192 x 12288: fp16 to powers of two 53 us (47 by bytes), bf16 with exact scales 70 us, where the seven operations of quotient()
 // for every value share the bound with the bytes.
 struct QuantArgs {
     const void* x;
@@ -69,6 +69,7 @@ void quantize_rows_kernel(const QuantArgs p)
         const int k0 = b * kBlock + lane8 * 16;
         const T* x = reinterpret_cast<const T*>(p.x) + src * p.x_stride + k0;
         float v[16];
+        uint32_t m = 0;                                             // magnitudes as integers: NaN is the largest
         if (live && ALIGN && k0 < p.K)                              // K % 16 == 0
         {
             __align__(16) uint32_t w[4 * sizeof(T)];
@@ -78,15 +79,26 @@ void quantize_rows_kernel(const QuantArgs p)
             const T* h = reinterpret_cast<const T*>(w);
             #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = to_float(h[i]);
+            if constexpr (sizeof(T) == 2)
+            {
+                // 16-bit magnitudes two at a time: 12 instructions instead of 32
+                uint32_t m2 = 0;
+                #pragma unroll
+                for (int i = 0; i < 8; i += 2) m2 = __vimax3_u16x2(m2, w[i] & 0x7fff7fffu, w[i + 1] & 0x7fff7fffu);
+                const uint16_t top = (uint16_t) max(m2 & 0xffffu, m2 >> 16);
+                T t;
+                memcpy(&t, &top, 2);
+                m = __float_as_uint(to_float(t));
+            }
         }
         else
         {
             #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] = !ALIGN && live && k0 + i < p.K ? to_float(x[i]) : 0.0f;
         }
-        uint32_t m = 0;                                             // magnitudes as integers: NaN is the largest
-        #pragma unroll
-        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        if (!ALIGN || sizeof(T) == 4)
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
         #pragma unroll
         for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (!live) continue;

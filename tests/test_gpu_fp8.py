@@ -441,3 +441,23 @@ def test_both_sides_of_the_rule_for_few_tokens(ext, cuda_device, T):
         x = rows(T, d, torch.bfloat16, dev, 3)
         assert rel(exl3_fp8.fp8_mlp_prefill(x, L, LIMIT), ref_mlp(x, L, 0)) <= MLP_REL
     assert ext.read_status(dev) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_quantize_rows_non_finite_halves(ext, cuda_device, dtype):
+    """16-bit rows with a NaN or inf of either sign in one place of a block: that block has no finite value, the others
+    stay exact."""
+    dev = cuda_device
+    clean = rows(24, 512, dtype, dev, 5)
+    want_q, want_s = exl3_fp8.quantize_rows(clean)
+    for value in (float("nan"), float("inf"), -float("inf")):
+        x = clean.clone()
+        for r in range(24):
+            x[r, 128 + (r * 53) % 128] = value
+        q, s = exl3_fp8.quantize_rows(x)
+        deq = q.float() * s.repeat_interleave(128, 1)
+        assert bool(torch.isnan(deq[:, 128:256]).all())
+        keep = torch.ones(512, dtype=torch.bool, device=dev)
+        keep[128:256] = False
+        assert torch.equal(q.view(torch.uint8)[:, keep], want_q.view(torch.uint8)[:, keep])
+        assert torch.equal(s[:, [0, 2, 3]], want_s[:, [0, 2, 3]])
