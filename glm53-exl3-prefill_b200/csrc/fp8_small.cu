@@ -7,11 +7,11 @@
 // to a CTA's warps, whose sums are added in a fixed order at the end.  What counts is the number of warps that wait for memory:
 // one block in flight in each of 32 warps per SM beats four in each of 16 (6.4 against 8.4 us for one token,
 // 4096 x 4096, whose bytes take 2.6 us); neither rows copied to shared memory by the bulk-copy engine nor fp16
-// products were faster.  One launch does everything:
-//   one token   rows are quantised on the way: a warp reads a block's 128 values (4 a lane), takes their maximum, rounds
-//               them, and hands the words to the lanes whose fragment they belong to;
-//   2..16       (linear) rows are quantised by their own kernel first and read as fragments from L2.
-// The tcgen05 kernel needs 128 x 256 tiles and a pipeline to start up: 20 us for one token and 4096 x 4096, where the
+// products were faster, and prefetching a CTA's weight rows into L2 was slower (eight routes 45 us instead of 39).
+//   one token of a projection, routes   rows are quantised on the way: a warp reads a block's 128 values (4 a lane), takes their
+//               maximum, rounds them, and hands the words to the lanes whose fragment they belong to;
+//   up to 16 tokens, plain MLPs         rows are quantised by their own kernel first and read as fragments from L2.
+// The tcgen05 kernel needs 128 x 256 tiles and a pipeline to start up: 13 us for two tokens and 4096 x 4096 (5.7 here), whose
 // bytes take 2.6 us.
 #include "fp8_common.cuh"
 
@@ -169,7 +169,7 @@ __device__ __forceinline__ void stream_token(const uint8_t* const (&row)[NR][2],
 struct SmallLinearArgs {
     const void* x;
     int vec;
-    const uint8_t* q; int64_t q_stride;         // 2..16 tokens: quantised rows and their scales
+    const uint8_t* q; int64_t q_stride;         // 1..16 tokens: quantised rows and their scales
     const float* sx; int64_t sx_row, sx_blk;
     int T, N, K;
     const uint8_t* w; int64_t w_stride;
@@ -227,7 +227,7 @@ void linear_token_kernel(const SmallLinearArgs p)
     }
 }
 
-// 2..16 tokens: NG groups of 8 columns.
+// 1..16 tokens: NG groups of 8 columns.
 template <int NG, int WARPS, bool ALIGNED32>
 __global__ __launch_bounds__(WARPS * 32, 2)
 void linear_tokens_kernel(const SmallLinearArgs p)
