@@ -133,13 +133,14 @@ __device__ __forceinline__ double exact_inverse_sum(const RouteLogitsArgs& p, co
     return 1.0 / warp_sum(z);
 }
 
-// The candidates, one per lane (expert mine, -1 past n of them; every other expert's score is clearly below the last
-// chosen one), ranked by their scores in 64 bits: lane j < topk returns the expert of slot j.
+// The candidates, one per lane (expert mine, -1 past n of them and where fewer experts than slots are left; every other
+// expert's score is clearly below the last chosen one), ranked by their scores in 64 bits: lane j < topk returns the
+// expert of slot j.  A lane without an expert counts as -inf, which no expert's score is, so empty slots come last.
 template <bool SOFTMAX, class Tl>
 __device__ __noinline__ int rank_in_64_bits(const RouteLogitsArgs& p, const Tl* row, float m, int lane, int mine, int n)
 {
     const double inv = SOFTMAX ? exact_inverse_sum(p, row, m, lane) : 1.0;
-    const double c = mine >= 0 ? exact_score<SOFTMAX>(p, load_logit(row + mine), mine, m, inv) : 0.0;
+    const double c = mine >= 0 ? exact_score<SOFTMAX>(p, load_logit(row + mine), mine, m, inv) : -(double) INFINITY;
     int rank = 0;
     for (int j = 0; j < n; ++j)
     {

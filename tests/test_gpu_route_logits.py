@@ -183,3 +183,24 @@ def test_offsets_past_32_bits(ext, cuda_device):
     tail_ids, tail_w = exl3_router.LogitsRouter(2).route(logits[-7:])
     assert torch.equal(ids[-7:], tail_ids) and torch.equal(w[-7:], tail_w)
     check(logits[-7:], None, 2)
+
+
+@pytest.mark.parametrize("G,keep", [(1, 1), (4, 2)])
+def test_missing_slots_come_last_whatever_the_scores(ext, cuda_device, G, keep):
+    """Fewer experts than slots, with scores plus bias at or below zero, tied and not: experts first, then -1."""
+    E, k = 48, 6
+    few = [(1, 3), (0, 5, 9), (2, 4, 7, 11), (1, 2, 3, 4, 5)]
+    logits = torch.full((8, E), -float("inf"), device=cuda_device)
+    for t in range(8):
+        live = torch.tensor(few[t % 4], device=cuda_device)
+        logits[t, live] = 0.25 if t < 4 else torch.linspace(-1, 1, live.numel(), device=cuda_device)
+    flat = torch.full((E,), -1.0, device=cuda_device)
+    tied_above = flat.clone()                                # a tie of positive scores before a negative one
+    tied_above[1:3] = 0.5
+    sunk = logits.clone()                                    # scores of exactly zero
+    sunk[logits > -float("inf")] = -1e4
+    for scoring in ("sigmoid", "softmax"):
+        for l, b in ((logits, flat), (logits, tied_above), (logits, -0.25 - torch.arange(E, device=cuda_device) / 64),
+                     (sunk, torch.zeros_like(flat))):
+            ids, w = check(l, b.float(), k, scoring, G, keep)
+            assert ids[0].tolist()[2:] == [-1] * 4 and w[0].tolist()[2:] == [0.0] * 4
