@@ -331,8 +331,8 @@ __device__ __forceinline__ float weight_of(const SmallExpertArgs& p, int64_t slo
 
 // Gate and up rows n0 .. n0 + 15 of the expert of route blockIdx.y: act = silu(min(g, L)) * clamp(u, -L, L), fp32.
 // Two CTAs an SM, without spills: 8 / 16 routes of 4096 x 1536 in 39.1 / 72.4 us; three, with spills, 39.4 / 74.0; gate and up
-// rows in different warps, four CTAs, 40.5 / 70.
-template <class T>
+// rows in different warps, four CTAs, 40.5 / 70.  ALIGNED32: the weights start on 32 bytes (rows are multiples of 128).
+template <bool ALIGNED32, class T>
 __global__ __launch_bounds__(S_THREADS, 2)
 void gate_up_token_kernel(const SmallExpertArgs p)
 {
@@ -349,7 +349,7 @@ void gate_up_token_kernel(const SmallExpertArgs p)
                                       {w + (int64_t) (p.f + n0 + g) * p.d, w + (int64_t) (p.f + n0 + g + 8) * p.d}};
     const float* const sw[2] = {s + (n0 / kBlock) * nkb, s + ((p.f + n0) / kBlock) * nkb};
     float acc[2][2];
-    stream_token<2, true>(row, sw, reinterpret_cast<const T*>(p.x) + slot / p.topk * p.x_stride, p.vec != 0, p.d,
+    stream_token<2, ALIGNED32>(row, sw, reinterpret_cast<const T*>(p.x) + slot / p.topk * p.x_stride, p.vec != 0, p.d,
                              warp * nkb / S_WARPS, (warp + 1) * nkb / S_WARPS, lane, acc);
     if ((lane & 3) == 0)
         #pragma unroll
@@ -374,6 +374,7 @@ void gate_up_token_kernel(const SmallExpertArgs p)
 
 // Output columns n0 .. n0 + 15 of token blockIdx.y: the activations quantised on the way, every route's product, and their
 // weighted sum in slot order.  The (route, part of K) units of a token are dealt to the warps.
+template <bool ALIGNED32>
 __global__ __launch_bounds__(T_THREADS, 2)
 void down_token_kernel(const SmallExpertArgs p)
 {
@@ -391,7 +392,7 @@ void down_token_kernel(const SmallExpertArgs p)
         const uint8_t* const row[1][2] = {{w + (int64_t) (n0 + g) * p.f, w + (int64_t) (n0 + g + 8) * p.f}};
         const float* const sw[1] = {p.s2 + (e * (p.d / kBlock) + n0 / kBlock) * nkb};
         float acc[1][2];
-        stream_token<1, true>(row, sw, p.act + slot * p.f, true, p.f, u % parts * nkb / parts,
+        stream_token<1, ALIGNED32>(row, sw, p.act + slot * p.f, true, p.f, u % parts * nkb / parts,
                                    (u % parts + 1) * nkb / parts, lane, acc);
         if ((lane & 3) == 0)
         {
@@ -472,14 +473,21 @@ int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_s
     p.w13 = static_cast<const uint8_t*>(w13); p.s13 = s13; p.w2 = static_cast<const uint8_t*>(w2); p.s2 = s2;
     p.limit = limit; p.act = act;
     p.out = out; p.out_dtype = out_dtype; p.out_stride = out_stride; p.accumulate = accumulate;
+    // (weights are 16-byte aligned, like those of the products by tiles)
     const dim3 grid((unsigned) (f / 16), (unsigned) (T * topk));
-    if (dtype == 0) gate_up_token_kernel<float><<<grid, S_THREADS, 0, stream>>>(p);
-    else if (dtype == 1) gate_up_token_kernel<__half><<<grid, S_THREADS, 0, stream>>>(p);
-    else gate_up_token_kernel<__nv_bfloat16><<<grid, S_THREADS, 0, stream>>>(p);
+    const bool a13 = reinterpret_cast<uintptr_t>(w13) % 32 == 0, a2 = reinterpret_cast<uintptr_t>(w2) % 32 == 0;
+    auto go = [&](auto v) {
+        using Tx = decltype(v);
+        if (a13) gate_up_token_kernel<true, Tx><<<grid, S_THREADS, 0, stream>>>(p);
+        else gate_up_token_kernel<false, Tx><<<grid, S_THREADS, 0, stream>>>(p);
+    };
+    if (dtype == 0) go(float{});
+    else if (dtype == 1) go(__half{});
+    else go(__nv_bfloat16{});
     int rc = check_launch("fp8_experts (gate and up, few routes)");
     if (rc) return rc;
-    return launch_after("fp8_experts (down, few routes)", down_token_kernel, dim3((unsigned) (d / 16), (unsigned) T),
-                        T_THREADS, 0, stream, p);
+    return launch_after("fp8_experts (down, few routes)", a2 ? down_token_kernel<true> : down_token_kernel<false>,
+                        dim3((unsigned) (d / 16), (unsigned) T), T_THREADS, 0, stream, p);
 }
 
 }  // namespace exl3b

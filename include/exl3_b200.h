@@ -266,8 +266,8 @@ EXL3_API int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K,
                              int64_t workspace_bytes, int32_t* status, void* stream);
 
 /* A gated MLP: out [T, d] (+)= quantised( silu(min(g, limit)) * clamp(u, -limit, limit) ) . w2^T with
- * g | u = quantised(x) . w13^T.  w13 e4m3 [2f, d] (gate rows, then up rows), w2 e4m3 [d, f], contiguous, scales
- * [2f / 128, d / 128] and [d / 128, f / 128].  d, f % 128 == 0. */
+ * g | u = quantised(x) . w13^T.  w13 e4m3 [2f, d] (gate rows, then up rows), w2 e4m3 [d, f], contiguous and 16-byte
+ * aligned, scales [2f / 128, d / 128] and [d / 128, f / 128].  d, f % 128 == 0. */
 EXL3_API int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f);
 EXL3_API int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_stride, const void* w13,
                           const float* w13_scale, const void* w2, const float* w2_scale, int64_t f, double limit,

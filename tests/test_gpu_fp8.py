@@ -461,3 +461,37 @@ def test_quantize_rows_non_finite_halves(ext, cuda_device, dtype):
         keep[128:256] = False
         assert torch.equal(q.view(torch.uint8)[:, keep], want_q.view(torch.uint8)[:, keep])
         assert torch.equal(s[:, [0, 2, 3]], want_s[:, [0, 2, 3]])
+
+
+def _at_16(t):
+    """A copy of `t` that starts 16 bytes behind a 32-byte boundary."""
+    flat = torch.empty(t.numel() + 64, dtype=torch.uint8, device=t.device)
+    start = (16 - flat.data_ptr()) % 32
+    view = flat[start:start + t.numel()].view(t.dtype).view(t.shape)
+    view.copy_(t)
+    assert view.data_ptr() % 32 == 16 and view.is_contiguous()
+    return view
+
+
+@pytest.mark.parametrize("T", [1, 3, 12, 40])
+def test_weights_aligned_to_16_bytes(ext, cuda_device, T):
+    """Weights cut out of one flat buffer start on 16 bytes, not 32: every path gives the same bits."""
+    dev = cuda_device
+    E, d, f, k = 24, 384, 256, 2
+    for bank in (make_layer(E, d, f, 121, dev), make_layer(1, d, f, 123, dev)):
+        n = bank.w13_fp8.shape[0]
+        ids, w = (t.to(dev) for t in synth.routing("uniform", T, n, min(k, n), seed=5))
+        for names in (("w13_fp8",), ("w2_fp8",), ("w13_fp8", "w2_fp8")):
+            moved = types.SimpleNamespace(**vars(bank))
+            for name in names:
+                setattr(moved, name, _at_16(getattr(bank, name)))
+            for dt in (torch.float32, torch.float16, torch.bfloat16):
+                x = rows(T, d, dt, dev, 2)
+                want = exl3_fp8.fp8_prefill(x, ids, w, bank, LIMIT)
+                assert rel(want, ref_experts(x, ids, w, bank)) <= MLP_REL
+                assert torch.equal(exl3_fp8.fp8_prefill(x, ids, w, moved, LIMIT), want)
+                if n == 1:
+                    assert torch.equal(exl3_fp8.fp8_mlp_prefill(x, moved, LIMIT), exl3_fp8.fp8_mlp_prefill(x, bank, LIMIT))
+                assert torch.equal(exl3_fp8.fp8_linear(x, moved.w13_fp8[0], bank.w13_scale[0]),
+                                   exl3_fp8.fp8_linear(x, bank.w13_fp8[0], bank.w13_scale[0]))
+    assert ext.read_status(dev) == 0
