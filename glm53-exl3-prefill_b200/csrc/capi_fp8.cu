@@ -28,10 +28,15 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes)
 
 constexpr int64_t kMaxDim = 0x7fffff00;
 
-// A piece of the caller's workspace, 256-byte aligned.
+// Pieces of the caller's workspace (null: only their sizes), 256-byte aligned whatever the workspace's own alignment of 16
+// bytes or more: kernels store whole 32-byte sectors into them.
+constexpr int64_t kAlignSlack = 256 - 16;
 struct Carver {
     uint8_t* base;
     int64_t used = 0;
+    explicit Carver(void* workspace)
+        : base(reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255))) {}
+    int64_t bytes() const { return used ? used + kAlignSlack : 0; }
     template <class T> T* take(int64_t n)
     {
         uint8_t* p = base ? base + used : nullptr;
@@ -262,10 +267,10 @@ int64_t exl3_fp8_linear_workspace(int64_t T, int64_t K, int64_t N)
         return -1;
     }
     if (T <= 1) return 0;                               // one row is quantised on the way
-    Carver c{nullptr};
+    Carver c(nullptr);
     take_rows(c, T, K);
     if (!few_tokens(T, N, K)) take_parts(c, T, 1, N, K);
-    return c.used;
+    return c.bytes();
 }
 
 int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t x_stride, const void* w, int64_t w_stride,
@@ -290,7 +295,7 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
     if (T == 1)
         return launch_fp8_linear_token(x, (int) dtype, (int) K, w, w_stride, w_scale, w_scale_stride, (int) N, out,
                                        (int) out_dtype, accumulate ? 1 : 0, as_stream(stream));
-    Carver c{static_cast<uint8_t*>(workspace)};
+    Carver c(workspace);
     const Rows8 r = take_rows(c, T, K);
     rc = launch_fp8_quantize(x, (int) dtype, T, (int) K, x_stride, 0, r.q, K, r.s, 1, T, nullptr, 1, nullptr,
                              false, as_stream(stream));
@@ -313,17 +318,17 @@ int exl3_fp8_linear(const void* x, int64_t dtype, int64_t T, int64_t K, int64_t 
 int64_t exl3_fp8_mlp_workspace(int64_t T, int64_t d, int64_t f)
 {
     if (check_experts_shape("fp8_mlp", T, 1, 1, d, f)) return -1;
-    Carver c{nullptr};
+    Carver c(nullptr);
     take_rows(c, T, d);
     take_rows(c, T, f);
     if (few_mlp_tokens(T, d, f))
     {
         c.take<float>(T * 2 * f);
-        return c.used;
+        return c.bytes();
     }
     take_parts(c, T, 1, 2 * f, d);
     take_parts(c, T, 1, d, f);
-    return c.used;
+    return c.bytes();
 }
 
 int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_stride, const void* w13,
@@ -340,7 +345,7 @@ int exl3_fp8_mlp(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_s
     if (!aligned16(w13) || !aligned16(w2)) return set_error("fp8_mlp: weights must be 16-byte aligned");
     if (!aligned16(workspace) || workspace_bytes < exl3_fp8_mlp_workspace(T, d, f))
         return set_error("fp8_mlp: workspace must hold exl3_fp8_mlp_workspace() bytes");
-    Carver c{static_cast<uint8_t*>(workspace)};
+    Carver c(workspace);
     const Rows8 xr = take_rows(c, T, d), hr = take_rows(c, T, f);
     if (few_mlp_tokens(T, d, f))
     {
@@ -376,9 +381,9 @@ int64_t exl3_fp8_experts_workspace(int64_t T, int64_t topk, int64_t E, int64_t d
 {
     if (check_experts_shape("fp8_experts", T, topk, E, d, f)) return -1;
     if (few_routes(T * topk, E)) return up256(T * topk * f * (int64_t) sizeof(float));
-    Carver c{nullptr};
+    Carver c(nullptr);
     take_experts(c, T, topk, E, d, f);
-    return c.used;
+    return c.bytes();
 }
 
 int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t x_stride, const void* ids,
@@ -405,7 +410,7 @@ int exl3_fp8_experts(const void* x, int64_t dtype, int64_t T, int64_t d, int64_t
                                         (int) weight_dtype, (int) topk, (int) E, w13, w13_scale, w2, w2_scale, (int) f,
                                         (float) limit, static_cast<float*>(workspace), out, (int) out_dtype, out_stride,
                                         accumulate ? 1 : 0, st);
-    Carver c{static_cast<uint8_t*>(workspace)};
+    Carver c(workspace);
     const ExpertBuffers b = take_experts(c, T, topk, E, d, f);
     // sorted by routing slot t * topk + j, so that each row knows both its token and its place in y
     rc = launch_route_sort(ids, ids_is_int64 ? 1 : 0, weights, (int) weight_dtype, R, 1, (int) E, 0, b.slot,

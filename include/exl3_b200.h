@@ -248,7 +248,8 @@ EXL3_API int exl3_route_logits(const void* logits, int64_t dtype, int64_t T, int
  * 8-bit layers (no reference counterpart): weights in e4m3 with one fp32 scale per block of 128 x 128, the
  * activations quantised to e4m3 with one fp32 scale per row and 128 columns:
  *   s = max(|x| over the block, 2^-64) / 448 (pow2: the least power of two at or above that), q = e4m3(x / s).
- * A block that holds NaN or inf gives NaN.  dtype codes: EXL3_DTYPE_*; strides in elements.
+ * A block that holds NaN or inf gives NaN.  dtype codes: EXL3_DTYPE_*; strides in elements.  Workspaces are the caller's,
+ * 16-byte aligned, of the bytes that the *_workspace call gives for the same sizes.
  * ------------------------------------------------------------------------------------------- */
 
 /* q e4m3 [rows, K] (row stride q_stride), scale fp32: block b of row r at scale[r * s_row + b * s_blk]. */

@@ -495,3 +495,41 @@ def test_weights_aligned_to_16_bytes(ext, cuda_device, T):
                 assert torch.equal(exl3_fp8.fp8_linear(x, moved.w13_fp8[0], bank.w13_scale[0]),
                                    exl3_fp8.fp8_linear(x, bank.w13_fp8[0], bank.w13_scale[0]))
     assert ext.read_status(dev) == 0
+
+
+@pytest.mark.parametrize("shift", [16, 48, 240])
+def test_workspaces_aligned_to_16_bytes(ext, cuda_device, shift):
+    """The C calls take a workspace at any multiple of 16 and write nothing past the size they asked for.  Wide tiles with
+    activations (whole-sector stores), split products, and the kernels for few tokens."""
+    dev, lib = cuda_device, ext.load()
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    status = ext.status_tensor(dev).data_ptr()
+
+    def shifted(need):
+        flat = torch.full((need + 1024,), 85, dtype=torch.uint8, device=dev)
+        start = -flat.data_ptr() % 256 + shift
+        return flat, start, flat.data_ptr() + start
+
+    for T, d, f, E, k in ((300, 256, 128, 4, 2), (60, 1024, 512, 2, 2), (9, 256, 128, 2, 2)):
+        L = make_layer(E, d, f, 131, dev)
+        x = rows(T, d, torch.float32, dev, 4)
+        ids, w = (t.to(dev) for t in synth.routing("uniform", T, E, k, seed=5))
+        one = types.SimpleNamespace(w13_fp8=L.w13_fp8[:1], w13_scale=L.w13_scale[:1], w2_fp8=L.w2_fp8[:1], w2_scale=L.w2_scale[:1])
+        ptrs = [t.data_ptr() for t in (L.w13_fp8, L.w13_scale, L.w2_fp8, L.w2_scale)]
+        calls = [(exl3_fp8.fp8_mlp_prefill(x, one, LIMIT), lib.exl3_fp8_mlp_workspace(T, d, f),
+                  lambda out, ws, n: lib.exl3_fp8_mlp(x.data_ptr(), 0, T, d, d, *ptrs, f, LIMIT, out, 0, d, 0, ws, n, status,
+                                                      stream)),
+                 (exl3_fp8.fp8_prefill(x, ids, w, L, LIMIT), lib.exl3_fp8_experts_workspace(T, k, E, d, f),
+                  lambda out, ws, n: lib.exl3_fp8_experts(x.data_ptr(), 0, T, d, d, ids.data_ptr(), 1, w.data_ptr(), 0, k, E,
+                                                          *ptrs, f, LIMIT, out, 0, d, 0, ws, n, status, stream)),
+                 (exl3_fp8.fp8_linear(x, L.w13_fp8[0], L.w13_scale[0]), lib.exl3_fp8_linear_workspace(T, d, 2 * f),
+                  lambda out, ws, n: lib.exl3_fp8_linear(x.data_ptr(), 0, T, d, d, ptrs[0], d, ptrs[1], d // 128, 2 * f, out, 0,
+                                                         2 * f, 0, ws, n, status, stream))]
+        assert w.dtype == torch.float32 and ids.dtype == torch.int64
+        for want, need, call in calls:
+            flat, start, ws = shifted(need)
+            out = torch.empty_like(want)
+            assert call(out.data_ptr(), ws, need) == 0, lib.exl3_last_error()
+            assert torch.equal(out, want)
+            assert bool((flat[:start] == 85).all()) and bool((flat[start + need:] == 85).all())
+    assert ext.read_status(dev) == 0
