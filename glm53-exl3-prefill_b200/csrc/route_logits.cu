@@ -206,11 +206,11 @@ __device__ __noinline__ int select_in_64_bits(const RouteLogitsArgs& p, const Tl
     return mine;
 }
 
-// The groups kept (a bit each) by their scores, from the token's selection scores sc[E] in shared memory; `gap`: how far
-// the last kept group's score is above the best dropped one's, and `low` the former.  lanes_per_group lanes scan a group and
-// merge their two best.
+// The groups kept (a bit each) by their scores, from the token's selection scores sc[E] in shared memory.  `tie`: whether a kept
+// group's score may really be below a dropped one's, each score being off by up to kTol times (1 + its addends'
+// magnitudes): two of opposite sign may cancel in the sum, their roundings do not.  lanes_per_group lanes scan a group and merge their two best.
 template <class F>
-__device__ __forceinline__ unsigned kept_groups(const RouteLogitsArgs& p, const F* sc, int lane, F& low, F& gap)
+__device__ __forceinline__ unsigned kept_groups(const RouteLogitsArgs& p, const F* sc, int lane, bool& tie)
 {
     const int lpg = p.lanes_per_group, g = lane / lpg, sub = lane - g * lpg;
     F b1 = lowest<F>(), b2 = lowest<F>();
@@ -227,20 +227,25 @@ __device__ __forceinline__ unsigned kept_groups(const RouteLogitsArgs& p, const 
         b2 = max(min(b1, o1), max(b2, o2));
         b1 = max(b1, o1);
     }
-    const F mine = g < p.n_group ? (p.group_top > 1 ? b1 + b2 : b1) : lowest<F>();
-    const F gs = __shfl_sync(kFull, mine, (lane * lpg) & 31);               // lane g: group g
+    if (p.group_top == 1) b2 = F(0);
+    const F gs = __shfl_sync(kFull, b1 + b2, (lane * lpg) & 31);      // lane g: group g
     int rank = 0;
     for (int o = 0; o < p.n_group; ++o)
     {
         const F x = __shfl_sync(kFull, gs, o);
         rank += x > gs || (x == gs && o < lane);
     }
-    const bool is_group = lane < p.n_group;
-    const unsigned last = __ballot_sync(kFull, is_group && rank == p.topk_group - 1);
-    const unsigned next = __ballot_sync(kFull, is_group && rank == p.topk_group);
-    low = __shfl_sync(kFull, gs, __ffs(last) - 1);
-    gap = low - __shfl_sync(kFull, gs, __ffs(next) - 1);
-    return __ballot_sync(kFull, is_group && rank < p.topk_group);
+    const bool is_group = lane < p.n_group, is_kept = is_group && rank < p.topk_group;
+    if constexpr (std::is_same_v<F, float>)
+    {
+        // a group without the experts for its score is at -inf, above or below which nothing is in doubt
+        const float mag = __shfl_sync(kFull, fabsf(b1) + fabsf(b2), (lane * lpg) & 31);
+        const float err = gs > -INFINITY ? kTol * (1.0f + mag) : 0.0f;
+        const uint32_t low = __reduce_min_sync(kFull, is_kept ? order_key(gs - err) : kFull);
+        const uint32_t next = __reduce_max_sync(kFull, is_group && !is_kept ? order_key(gs + err) : 0u);
+        tie = next >= low && low > order_key(-INFINITY);
+    }
+    return __ballot_sync(kFull, is_kept);
 }
 
 // The same from scores in 64 bits, which replace sc.
@@ -256,8 +261,8 @@ __device__ __noinline__ unsigned kept_groups_in_64_bits(const RouteLogitsArgs& p
         sc[e] = l > -INFINITY && c > lowest<double>() ? c : lowest<double>();
     }
     __syncwarp();
-    double low, gap;
-    return kept_groups<double>(p, sc, lane, low, gap);
+    bool tie;
+    return kept_groups<double>(p, sc, lane, tie);
 }
 
 // CTAs that an SM holds at a time (64, 80 or 128 registers a thread).
@@ -328,11 +333,9 @@ void route_logits_kernel(const __grid_constant__ RouteLogitsArgs p)
                 sc[e] = c;
             }
             __syncwarp();
-            float low, gap;
-            kept = kept_groups<float>(p, sc, lane, low, gap);
-            // a group's score is a sum of up to two: twice the error of one.  (A group without two experts left is at
-            // -inf, and a gap of nothing to -inf is no near-tie.)
-            if ((by_score || sums) && gap <= 2.0f * kTol * (1.0f + fabsf(low)) && low > -INFINITY)
+            bool tie;
+            kept = kept_groups<float>(p, sc, lane, tie);
+            if ((by_score || sums) && tie)
                 kept = kept_groups_in_64_bits<SOFTMAX, Tl>(p, row, m, lane, s_rows + warp * p.E);
             #pragma unroll
             for (int i = 0; i < MPL; ++i)

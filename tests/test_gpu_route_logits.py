@@ -204,3 +204,15 @@ def test_missing_slots_come_last_whatever_the_scores(ext, cuda_device, G, keep):
                      (sunk, torch.zeros_like(flat))):
             ids, w = check(l, b.float(), k, scoring, G, keep)
             assert ids[0].tolist()[2:] == [-1] * 4 and w[0].tolist()[2:] == [0.0] * 4
+
+
+def test_group_scores_of_cancelling_biases(ext, cuda_device):
+    """The two best of a group have large biases of opposite sign: their sum is small and its rounding is not."""
+    dev = cuda_device
+    g = torch.Generator(device=dev).manual_seed(19)
+    noise = torch.randn(300, 16, generator=g, device=dev)
+    for sizes in ([64.0] * 8, [1000.0] * 8, [0.0, 64.0, 1000.0, 3e4, 0.0, 64.0, 1000.0, 3e4]):
+        bias = torch.tensor([v for s in sizes for v in (s, -s)], device=dev)
+        for spread in (1e-5, 1e-4, 1e-3):                    # about the rounding of the addends, and on both sides of it
+            for scoring in ("sigmoid", "softmax"):
+                check(0.3 + spread * noise, bias, 5, scoring, n_group=8, topk_group=3)
