@@ -206,9 +206,11 @@ __device__ __noinline__ int select_in_64_bits(const RouteLogitsArgs& p, const Tl
     return mine;
 }
 
-// The groups kept (a bit each) by their scores, from the token's selection scores sc[E] in shared memory.  `tie`: whether a kept
-// group's score may really be below a dropped one's, each score being off by up to kTol times (1 + its addends'
-// magnitudes): two of opposite sign may cancel in the sum, their roundings do not.  lanes_per_group lanes scan a group and merge their two best.
+// The groups kept (a bit each) by their scores, from the token's selection scores sc[E] in shared memory.  A group's score is
+// taken as half of its definition's (a mean where two are summed): the order is the same and no sum overflows.  `tie`:
+// whether a kept group's score may really be below a dropped one's, each score being off by up to kTol / 2 times (1 +
+// the mean of its addends' magnitudes): two of opposite sign may cancel in the sum, their roundings do not.
+// lanes_per_group lanes scan a group and merge their two best.
 template <class F>
 __device__ __forceinline__ unsigned kept_groups(const RouteLogitsArgs& p, const F* sc, int lane, bool& tie)
 {
@@ -227,8 +229,9 @@ __device__ __forceinline__ unsigned kept_groups(const RouteLogitsArgs& p, const 
         b2 = max(min(b1, o1), max(b2, o2));
         b1 = max(b1, o1);
     }
-    if (p.group_top == 1) b2 = F(0);
-    const F gs = __shfl_sync(kFull, b1 + b2, (lane * lpg) & 31);      // lane g: group g
+    if (p.group_top == 1) b2 = b1;
+    const F half1 = F(0.5) * b1, half2 = F(0.5) * b2;
+    const F gs = __shfl_sync(kFull, half1 + half2, (lane * lpg) & 31);      // lane g: group g
     int rank = 0;
     for (int o = 0; o < p.n_group; ++o)
     {
@@ -239,8 +242,8 @@ __device__ __forceinline__ unsigned kept_groups(const RouteLogitsArgs& p, const 
     if constexpr (std::is_same_v<F, float>)
     {
         // a group without the experts for its score is at -inf, above or below which nothing is in doubt
-        const float mag = __shfl_sync(kFull, fabsf(b1) + fabsf(b2), (lane * lpg) & 31);
-        const float err = gs > -INFINITY ? kTol * (1.0f + mag) : 0.0f;
+        const float mag = __shfl_sync(kFull, fabsf(half1) + fabsf(half2), (lane * lpg) & 31);
+        const float err = gs > -INFINITY ? 0.5f * kTol * (1.0f + mag) : 0.0f;
         const uint32_t low = __reduce_min_sync(kFull, is_kept ? order_key(gs - err) : kFull);
         const uint32_t next = __reduce_max_sync(kFull, is_group && !is_kept ? order_key(gs + err) : 0u);
         tie = next >= low && low > order_key(-INFINITY);

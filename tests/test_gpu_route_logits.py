@@ -216,3 +216,20 @@ def test_group_scores_of_cancelling_biases(ext, cuda_device):
         for spread in (1e-5, 1e-4, 1e-3):                    # about the rounding of the addends, and on both sides of it
             for scoring in ("sigmoid", "softmax"):
                 check(0.3 + spread * noise, bias, 5, scoring, n_group=8, topk_group=3)
+
+
+def test_group_scores_past_the_largest_float(ext, cuda_device):
+    """Sums of two biases that fp32 does not hold: groups keep their order, and finite ones stay above empty ones."""
+    dev = cuda_device
+    logits, bias = _logits(30, 16, torch.float32, dev, seed=23)
+    high = bias.clone()
+    high[0:4] = torch.tensor([3e38, 2e38, 1.0, 1.0], device=dev)
+    high[8:12] = torch.tensor([3e38, 2.5e38, 2.5e38, 1.0], device=dev)
+    low = bias.clone()
+    low[4:8], low[8:12] = torch.finfo(torch.float32).min, -3e38
+    empty = logits.clone()
+    empty[:, :4] = -float("inf")
+    for l in (logits, empty):
+        for b in (high, low):
+            for keep in (1, 2, 3):
+                check(l, b, 3, n_group=4, topk_group=keep)
