@@ -86,6 +86,8 @@ def grouped_prefill(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
     gp = _load_ext()
     dev = x2d.device
     T, K = x2d.shape
+    if ids.dim() != 2 or ids.shape[0] != T:                 # the sort's buffers are sized by x2d's rows
+        raise RuntimeError("ids / weights must be [T, topk], one row per row of x2d")
     topk = ids.shape[1]
     R = T * topk
     E = int(layer.w13_trellis.shape[0])

@@ -72,6 +72,8 @@ def moe_prefill_from_logits(x2d: torch.Tensor, logits: torch.Tensor, router: Log
     experts = layer.w13_fp8 if exl3_fp8.is_fp8_layer(layer) else layer.w13_trellis
     if logits.dim() == 2 and logits.shape[1] != experts.shape[0]:
         raise RuntimeError("the logits and the layer disagree on the number of experts")
+    if logits.dim() == 2 and logits.shape[0] != x2d.shape[0]:
+        raise RuntimeError("the logits and the hidden states disagree on the number of tokens")
     ids, w = router.route(logits)
     out = exl3_dense.moe_block_prefill(x2d, ids, w, layer, shared, limit)
     return (out, ids, w) if return_routing else out

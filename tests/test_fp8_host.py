@@ -208,3 +208,18 @@ def test_quantize_weight(shape):
         assert torch.allclose(s[..., 0, b] * 448, block.abs().amax(dim=(-2, -1)), rtol=1e-6, atol=1e-15)
     with pytest.raises(RuntimeError, match="NaN or inf"):
         exl3_fp8.quantize_weight(torch.full((2, 16), float("nan")))
+
+
+@pytest.mark.parametrize("rows", [3, 5])
+def test_routing_of_other_tokens_is_refused(lib, rows):
+    """Logits (or ids) for another number of tokens than the hidden states have, with either kind of layer."""
+    x = torch.zeros(4, 256)
+    fp8 = types.SimpleNamespace(w13_fp8=torch.zeros(8, 256, 256, dtype=torch.float8_e4m3fn), w13_scale=torch.ones(8, 2, 2),
+                                w2_fp8=torch.zeros(8, 256, 128, dtype=torch.float8_e4m3fn), w2_scale=torch.ones(8, 2, 1))
+    trellis = types.SimpleNamespace(w13_trellis=torch.zeros(8, 2, 16, 8, 64, dtype=torch.int16))
+    for layer in (fp8, trellis):
+        with pytest.raises(RuntimeError, match="number of tokens"):
+            exl3_router.moe_prefill_from_logits(x, torch.zeros(rows, 8), exl3_router.LogitsRouter(2), layer, 7.0)
+        for ids in (torch.zeros(rows, 2, dtype=torch.int64), torch.zeros(4, dtype=torch.int64)):
+            with pytest.raises(RuntimeError, match=r"\[T, topk\]"):
+                exl3_dense.moe_block_prefill(x, ids, torch.ones(ids.shape), layer, None, 7.0)
