@@ -69,7 +69,7 @@ def dense_mlp_prefill(x2d: torch.Tensor, mlp, limit: float, out: torch.Tensor | 
         hook("fp8_mlp")
         if out is not None and out.dtype != torch.float32:
             raise RuntimeError("dense_mlp_prefill: out must be fp32")
-        out = exl3_fp8.fp8_mlp_prefill(x2d, mlp, limit, out=out)
+        out = exl3_fp8.fp8_mlp_prefill(exl3_fp8.as_rows(x2d), mlp, limit, out=out)
         hook("end")
         return out
     if int(mlp.w13_trellis.shape[0]) != 1:

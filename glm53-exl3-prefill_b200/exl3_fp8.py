@@ -31,6 +31,15 @@ def is_fp8_layer(layer) -> bool:
     return getattr(layer, "w13_fp8", None) is not None
 
 
+def as_rows(x2d: torch.Tensor) -> torch.Tensor:
+    """x2d of any float type and strides as the kernels take it: fp32, fp16 or bf16 in contiguous, separate rows."""
+    if x2d.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        x2d = x2d.float()
+    if x2d.dim() == 2 and (x2d.shape[1] > 1 and x2d.stride(1) != 1 or x2d.shape[0] > 1 and x2d.stride(0) < x2d.shape[1]):
+        x2d = x2d.contiguous()
+    return x2d
+
+
 def quantize_rows(x2d: torch.Tensor, pow2: bool = False):
     """x2d [T, K] (fp32, fp16, bf16; rows may be strided) -> (q e4m3 [T, K], scale fp32 [T, ceil(K / 128)]).
     pow2 takes the least power of two at or above amax / 448 as the scale."""

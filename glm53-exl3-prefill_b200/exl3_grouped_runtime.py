@@ -78,7 +78,9 @@ def grouped_prefill(x2d: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
         if out is not None and out.dtype != torch.float32:
             raise RuntimeError("out must be a contiguous fp32 [T, K] tensor on the input's device")
         hook("fp8_experts")
-        out = exl3_fp8.fp8_prefill(x2d, ids, weights, layer, limit, out=out)
+        if weights.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            weights = weights.float()
+        out = exl3_fp8.fp8_prefill(exl3_fp8.as_rows(x2d), ids, weights, layer, limit, out=out)
         hook("end")
         return out
     if deterministic is None:

@@ -533,3 +533,20 @@ def test_workspaces_aligned_to_16_bytes(ext, cuda_device, shift):
             assert torch.equal(out, want)
             assert bool((flat[:start] == 85).all()) and bool((flat[start + need:] == 85).all())
     assert ext.read_status(dev) == 0
+
+
+def test_shared_entry_points_take_any_float_type_and_strides(ext, cuda_device):
+    """grouped_prefill and its kin take 8-bit layers on the inputs that they take trellis layers on: 64-bit values and
+    weights, strided columns, broadcast rows."""
+    dev = cuda_device
+    T, E, d, f, k = 30, 6, 256, 128, 2
+    L, S = make_layer(E, d, f, 141, dev), make_layer(1, d, f, 143, dev)
+    ids, w = (t.to(dev) for t in synth.routing("uniform", T, E, k, seed=5))
+    x = rows(T, d, torch.float32, dev, 4)
+    want = exl3_dense.moe_block_prefill(x, ids, w, L, S, LIMIT)
+    assert rel(want, ref_experts(x, ids, w, L) + ref_mlp(x, S, 0)) <= MLP_REL
+    for same in (x.double(), x.t().contiguous().t()):
+        assert torch.equal(exl3_dense.moe_block_prefill(same, ids, w.double(), L, S, LIMIT), want)
+    one = x[:1].expand(T, d)
+    assert torch.equal(exl3_dense.moe_block_prefill(one, ids, w, L, S, LIMIT),
+                       exl3_dense.moe_block_prefill(one.contiguous(), ids, w, L, S, LIMIT))
