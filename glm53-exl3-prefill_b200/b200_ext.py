@@ -140,8 +140,8 @@ def status_tensor(dev: torch.device) -> torch.Tensor:
     key = (dev.type, dev.index if dev.index is not None else torch.cuda.current_device())
     t = _status.get(key)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=dev)
-        _status[key] = t
+        # (of two threads that make one, both get the one that is kept)
+        t = _status.setdefault(key, torch.zeros(1, dtype=torch.int32, device=dev))
     return t
 
 

@@ -223,3 +223,22 @@ def test_routing_of_other_tokens_is_refused(lib, rows):
         for ids in (torch.zeros(rows, 2, dtype=torch.int64), torch.zeros(4, dtype=torch.int64)):
             with pytest.raises(RuntimeError, match=r"\[T, topk\]"):
                 exl3_dense.moe_block_prefill(x, ids, torch.ones(ids.shape), layer, None, 7.0)
+
+
+def test_two_threads_share_one_status_word(monkeypatch):
+    """First calls from two threads at once: both get the word that read_status reads (its address is kept)."""
+    import threading
+    together, made = threading.Barrier(2, timeout=20), torch.zeros
+
+    def zeros(*args, **kwargs):
+        together.wait()
+        return made(*args, **kwargs)
+    monkeypatch.setattr(b200_ext.torch, "zeros", zeros)
+    monkeypatch.setattr(b200_ext, "_status", {})
+    dev, got = torch.device("cpu", 0), []
+    threads = [threading.Thread(target=lambda: got.append(b200_ext.status_tensor(dev))) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 2 and got[0] is got[1] and got[0] is b200_ext.status_tensor(dev)
