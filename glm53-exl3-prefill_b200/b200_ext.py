@@ -140,8 +140,15 @@ def status_tensor(dev: torch.device) -> torch.Tensor:
     key = (dev.type, dev.index if dev.index is not None else torch.cuda.current_device())
     t = _status.get(key)
     if t is None:
-        # (of two threads that make one, both get the one that is kept)
-        t = _status.setdefault(key, torch.zeros(1, dtype=torch.int32, device=dev))
+        if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            # the graph's memory, which stays while the word does, but zeroed now on a stream outside the capture: a fill
+            # in the graph would reset the word at every replay
+            t = torch.empty(1, dtype=torch.int32, device=dev)
+            with torch.cuda.stream(torch.cuda.Stream(dev)):
+                t.zero_()
+        else:
+            t = torch.zeros(1, dtype=torch.int32, device=dev)
+        t = _status.setdefault(key, t)                      # of two threads that make one, both get the one that is kept
     return t
 
 

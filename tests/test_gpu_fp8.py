@@ -8,6 +8,9 @@
 * gated MLP: an activation within that error of a border between two e4m3 values may round to the other one.
   The error is below 2e-5 of the block's maximum for the K here, an e4m3 step is 2^-4 .. 2^-3 of a value, so at most
   about 1e-3 of the values flip, by 2^-3 each: sqrt(1e-3) * 2^-3 / 2 = 2e-3 of the result (2-norm)."""
+import os
+import subprocess
+import sys
 import types
 
 import numpy as np
@@ -550,3 +553,31 @@ def test_shared_entry_points_take_any_float_type_and_strides(ext, cuda_device):
     one = x[:1].expand(T, d)
     assert torch.equal(exl3_dense.moe_block_prefill(one, ids, w, L, S, LIMIT),
                        exl3_dense.moe_block_prefill(one.contiguous(), ids, w, L, S, LIMIT))
+
+
+def test_a_capture_as_the_first_call_keeps_the_status_word(ext, cuda_device):
+    """In a process whose first call is captured: the word exists, zeroed, outside the graph, and a replay does not reset
+    what an earlier launch recorded."""
+    code = """
+import sys
+sys.path.insert(0, {pkg!r})
+import torch, b200_ext, exl3_fp8
+dev = torch.device("cuda", 0)
+w, ws = exl3_fp8.quantize_weight(torch.randn(256, 256, generator=torch.Generator().manual_seed(1)))
+w, ws, x = w.to(dev), ws.to(dev), torch.ones(40, 256, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = exl3_fp8.fp8_linear(x, w, ws)
+torch.cuda.synchronize()
+assert b200_ext.read_status(dev) == 0
+b200_ext.status_tensor(dev).fill_(1)
+graph.replay()
+torch.cuda.synchronize()
+assert b200_ext.read_status(dev) == 1, "the replay reset the word"
+graph.replay()
+assert torch.equal(out, exl3_fp8.fp8_linear(x, w, ws)) and b200_ext.read_status(dev) == 0
+"""
+    pkg = os.path.dirname(os.path.abspath(exl3_fp8.__file__))
+    r = subprocess.run([sys.executable, "-c", code.format(pkg=pkg)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
