@@ -119,7 +119,10 @@ ExpertBuffers take_experts(Carver& c, int64_t T, int64_t topk, int64_t E, int64_
 
 // Routes whose products each read their expert's weights for themselves (fp8_small.cu), activations [R, f] in the workspace.
 // With 288 experts of 4096 x 1536 (every route another expert), 8 / 16 / 32 / 64 routes: 39 / 72 / 126 / 257 us, and 58 / 95 /
-// 138 / 203 us by the tiles of fp8_gemm.cu; where routes share experts the tiles read the weights once, hence the second bound.
+// 138 / 203 us by the tiles of fp8_gemm.cu.  Where routes share experts the tiles read their weights once, hence the second bound:
+// small experts gain up to it (1024 x 512: 24 routes over 24 experts 18.5 us, by tiles 30, which need 28 to start up; 2048 x 768:
+// 32 over 48 48 and 50 us), large ones only to about R * R = 12 E (4096 x 1536: 8 over 4 38 and 41 us, 16 over 8 68 and 56,
+// 32 over 16 126 and 86).
 bool few_routes(int64_t R, int64_t E) { return R <= 32 && R <= 2 * E; }
 
 // Tokens whose product streams the weights through fp8_small.cu rather than in tiles.  Up to 8 tokens it is never slower: 6.5

@@ -215,7 +215,7 @@ constexpr int kFp8FewTokens = 16;      // most rows of launch_fp8_linear_tokens
 int launch_fp8_linear_token(const void* x, int dtype, int K, const void* w, int64_t w_stride, const float* sw, int64_t sw_n,
                             int N, void* out, int out_dtype, int accumulate, cudaStream_t stream);
 int launch_fp8_linear_tokens(const Fp8GemmProblem& p, cudaStream_t stream);
-// ids, weights null: a plain MLP (topk 1, one expert, weight 1).
+// T * topk routes, each reading its expert's weights for itself; act: fp32 [T * topk, f] of scratch, 16-byte aligned.
 int launch_fp8_experts_small(const void* x, int dtype, int T, int d, int64_t x_stride, const void* ids, int ids_i64,
                              const void* weights, int wdtype, int topk, int E, const void* w13, const float* s13,
                              const void* w2, const float* s2, int f, float limit, float* act, void* out, int out_dtype,

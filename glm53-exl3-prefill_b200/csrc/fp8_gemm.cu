@@ -29,7 +29,8 @@
 // the loop is the way round one TMEM buffer (MMA, commit, taking the sums out, arrival, next MMA: about 2000 clocks),
 // and the two halves go round out of step.  A 256 x 256 x 128 block takes the pair about 1050 clocks, of which the MMAs
 // need 512, and the end of a tile about 5000, in which the tensor core waits (the sums are half of the register file, so there
-// is no second set): 8192 x 12288 x 4096 in 463 us, 53 % of twice the measured bf16 rate.  Eight epilogue warps with 64 columns
+// is no second set): 8192 x 12288 x 4096 in 463 us, 53 % of twice the measured bf16 rate, alone; 540..555 us, 45 %, call after
+// call, where the power cap lowers the clock.  Eight epilogue warps with 64 columns
 // each (spills: 562 us), all sixteen on each half in turn (553 us: more barriers a block) and spinning waits (511 us) were slower.
 //
 //   warp 0        TMA producer of this CTA's operands: weight blocks [128 x 128 B], token rows in boxes of 32;
@@ -959,9 +960,10 @@ int launch_fp8_gemm(const Fp8GemmProblem& q, cudaStream_t stream)
 
 int fp8_gemm_splits(int64_t rows, int n_experts, int N, int K)
 {
-    // the clusters of a B200 (148 SMs, some without a partner), the tiles there will be (an expert's last rows taken for
-    // a thin tile), and at least four K blocks a part: 777 x 576 x 4096 takes 22 us in six parts and 31 in one, 32 x 4096 x
-    // 4096 17 us in eight and 28 in one
+    // the clusters that run at one time (74 on a B200 whose SMs all have a partner, fewer where some do not; a constant, since a
+    // workspace's size does not depend on the device), the tiles there will be (an expert's last rows taken for a thin tile),
+    // and at least four K blocks a part: 777 x 576 x 4096 takes 22 us in six parts and 31 in one, 32 x 4096 x 4096 17 us in
+    // eight and 28 in one
     constexpr int64_t clusters = 72;
     const int64_t units = (N + 255) / 256, kb = (K + FG_BK - 1) / FG_BK;
     const int64_t experts = rows < n_experts ? rows : n_experts;

@@ -16,13 +16,15 @@
 // One warp per token: lane i holds experts i, i + 32, ... as keys (unsigned integers in the order of the floats) and
 // knows its two best; each of the topk rounds is two warp-wide integer reductions (the largest key, then the lowest
 // expert that holds it), after which the owner moves up its second best and only looks at its keys again when that is
-// gone too.  The bytes of the logits (33 MB for 32768 tokens of 256 experts, 5 us) bound it in principle; the instructions do
-// in fact, about 1100 a token: 8192 tokens of 288 experts take 14.4 us (1.6 by bytes), 32768 of 256 in 8 groups 56 us.
+// gone too.  The bytes of the logits (33 MB for 32768 tokens of 256 experts, 5 us) bound it in principle; the instructions and
+// the waits of one warp on its own loads and shuffles do in fact, about 870 instructions a token without groups and 1125 with:
+// 8192 tokens of 288 experts take 14.4 us (1.6 by bytes), 32768 of 256 in 8 groups 54 us.
 //
-// The choice is the one that exact arithmetic makes.  Without a bias both score functions grow with the
+// The choice is the one that 64-bit scores make.  Without a bias both score functions grow with the
 // logit, so experts are ranked by the logits themselves.  With a bias, scores in 32 bits rank them, and where two scores
 // that a decision separates are closer than that arithmetic can tell (kTol), the candidates, one a lane, are
-// ranked again by their scores in 64 bits; where two groups nearly tie, the groups are.
+// ranked again by their scores in 64 bits; where two groups nearly tie, the groups are.  Biased scores that are equal in
+// 64 bits are ties (sigmoids of logits above 37 all are 1 there).
 #include <cstdint>
 #include <type_traits>
 #include <cuda_bf16.h>

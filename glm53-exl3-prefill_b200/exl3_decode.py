@@ -13,8 +13,9 @@ its inputs into the bucket's buffers (padding tokens get expert id -1, which the
 replays the graph and returns a view of the bucket's fp32 output.  Results equal ``grouped_prefill``'s
 (bit for bit with deterministic=True; with the atomic down stage up to the order of the fp32 adds).  A layer of
 8-bit experts (exl3_fp8) is replayed alike; its inputs are held in fp32, so that any input type keeps its
-values, and results are those of grouped_prefill on the padded bucket (fp32 rounding apart from the same call
-without padding, which other kernels may take).
+values, and results are those of grouped_prefill on the padded bucket.  The same call without padding may take other
+kernels, whose sums run in another order: apart from fp32 rounding, an activation next to a border of two e4m3 values
+may then round to the other one.
 """
 from __future__ import annotations
 

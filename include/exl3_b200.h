@@ -233,7 +233,8 @@ EXL3_API int exl3_fat_gemm_scatter(const void* a, int64_t size_m, int64_t size_k
  *   a group's score is the sum of its group_top (1 or 2) largest c, over n_group equal groups of consecutive experts;
  *   ids = the topk experts by c inside the topk_group groups with the largest scores, best first;
  *   weights = s[ids] / (sum + 1e-20) if norm else s[ids], times scale.
- * Ties go to the lower expert (group), and the choice is that of exact arithmetic.  NaN and -inf logits are
+ * Ties go to the lower expert (group), and the choice is that of 64-bit scores (without a bias, experts rank by
+ * their logits).  NaN and -inf logits are
  * masked (never chosen; nor are experts with a NaN or -inf bias); missing experts give id -1 and weight 0.  logits
  * [T, E] of `dtype` with element stride row_stride between rows, bias fp32 [E] or NULL (+inf counts as the
  * largest float), ids int64 / weights fp32 [T, topk].
